@@ -27,6 +27,7 @@ extern "C" {
 #define RC_ERR_NOT_FOUND 2 /* unknown weight handle: the reference raises KeyError   */
 #define RC_ERR_CUDA 3      /* CUDA runtime failure: RuntimeError                      */
 #define RC_ERR_TIMEOUT 4   /* a bounded device-side wait ran out: RuntimeError        */
+#define RC_ERR_FULL 5      /* a KV page pool has no free page left: CacheFull         */
 
 #define RC_DTYPE_BF16 0
 #define RC_DTYPE_F32 1
@@ -365,6 +366,123 @@ int rc_add_bf16(rc_ctx *ctx, const uint16_t *a_dev, const uint16_t *b_dev, uint1
  * residual add followed by an RMS normalisation (no learned scale). */
 int rc_add_rms_bf16(rc_ctx *ctx, const uint16_t *a_dev, const uint16_t *b_dev, uint16_t *out_dev, int rows,
                     int n, float eps, void *stream);
+
+/* ------------------------------------------------------------ KV cache ---
+ * A paged cache of keys and values in q4nx groups (32 values: 4-bit codes,
+ * bf16 scale and min; 5 bits a value), and the attention that reads it.
+ * The pool is [layers][pages][kv_heads] head blocks; a head block holds
+ * page_size tokens as
+ *   K codes [page_size][D/2] | K params [page_size][D/32]{scale, min} |
+ *   V codes [page_size][D/2] | V params [page_size][D/32]{scale, min}
+ * and a value is min + scale * code.  Within a row of codes the 32-bit word
+ * q*(D/32)+j of a K row holds values 32j+8q .. 32j+8q+7, the 16-bit word
+ * g*(D/32)+j of a V row values 32j+4g .. 32j+4g+3, lower nibbles first: a
+ * lane of the attention kernels reads its share of a row in one load.
+ *
+ * A batch of sequences is described by device arrays: table [n_seqs][cols]
+ * with rows ld_table apart (page ids; token t of sequence s lies in page
+ * table[s][t / page_size]; entries past a sequence's tokens are not read),
+ * kv_len [n_seqs] (tokens of each sequence, those of this call included) and
+ * q_off [n_seqs + 1] (the rows of sequence s are q_off[s] .. q_off[s+1]-1;
+ * NULL: one row per sequence).  Row i of a sequence of n rows stands at
+ * position kv_len - n + i; a row whose position is negative is empty (an idle
+ * slot of a captured batch): it stores nothing and its attention is zero.
+ * Rows past q_off[n_seqs] are left alone.  max_q is an upper bound of the rows
+ * of a sequence, n_rows the rows the buffers hold.  Ids and lengths are read
+ * on the device: a page id outside the pool, or a length outside the table,
+ * sets the device error word (RC_ERR_INVALID at the next synchronising call)
+ * and the access is skipped. */
+typedef struct rc_kv rc_kv;
+
+/* Bytes of a pool.  head_dim is 64 or 128, page_size 16, 32, 64 or 128. */
+int rc_kv_pool_bytes(int layers, int pages, int kv_heads, int head_dim, int page_size, size_t *out);
+
+/* A cache on pool_dev (device memory of the caller, 16-byte aligned, at least
+ * rc_kv_pool_bytes long), or on memory of its own when pool_dev is NULL. */
+int rc_kv_create(rc_ctx *ctx, int layers, int pages, int kv_heads, int head_dim, int page_size, void *pool_dev,
+                 size_t pool_bytes, rc_kv **out);
+int rc_kv_destroy(rc_kv *kv);
+
+/* What lies between the q/k/v projection and the attention of one layer, in
+ * one pass.  x [n_rows][ldx] (RC_DTYPE_BF16 or RC_DTYPE_F32) holds q_heads
+ * query heads, then kv_heads key heads, then kv_heads value heads of head_dim
+ * values.  Query and key heads are RMS-normalised when q_norm / k_norm (bf16
+ * [head_dim]) are given, x / sqrt(mean(x^2) + eps) * w, and rotated when rope
+ * is given: rope [rope_rows][rope_dim] f32 holds cos | sin (rope_dim / 2 each)
+ * of a position; the first rope_dim values of a head turn in pairs
+ * (i, i + rope_dim/2), or (2i, 2i+1) when interleaved != 0; rope_dim is a
+ * multiple of 8, at most head_dim.  Queries go to q_out [n_rows][ldq] bf16;
+ * keys and values are quantised (the group rule of rc_quantize_q4nx: bf16
+ * floor of the minimum, bf16 ceiling of (max - min) / 15 stepped up until it
+ * covers the maximum, nearest code, ties to even), in 64 bits throughout, and
+ * stored at the row's position.  A group with a non-finite value or a range
+ * that overflows is stored as NaN and sets the device error word. */
+int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, int q_heads, int n_rows,
+                 const int32_t *table_dev, int cols, int ld_table, const int32_t *kv_len_dev,
+                 const int32_t *q_off_dev, int n_seqs, const uint16_t *q_norm_dev, const uint16_t *k_norm_dev, float eps,
+                 const float *rope_dev, int rope_rows, int rope_dim, int interleaved, uint16_t *q_out_dev, int ldq,
+                 void *stream);
+
+/* Attention of q [n_rows][ldq] (bf16, q_heads heads; consecutive
+ * q_heads / kv_heads query heads share a kv head) over the cache:
+ * out = sum_t softmax_t(scale * q . k_t) v_t over the tokens t <= p that the
+ * row at position p sees: all of them when window == 0, else those with
+ * t > p - window or t < sinks.  out [n_rows][ldo] bf16; zeros where a row sees
+ * nothing.  ldq and ldo are multiples of 8 and both buffers 16-byte aligned.
+ * A row's bytes do not depend on the other sequences of the batch.  Scratch
+ * grows on the first call for a larger batch or table (that call
+ * synchronises the device). */
+int rc_kv_attend(rc_kv *kv, int layer, const uint16_t *q_dev, int ldq, int q_heads, int n_rows,
+                 const int32_t *table_dev, int cols, int ld_table, const int32_t *kv_len_dev,
+                 const int32_t *q_off_dev, int n_seqs, int max_q, float scale, int window, int sinks, uint16_t *out_dev, int ldo,
+                 void *stream);
+
+/* The cached keys and values of the batch's rows, rounded to bf16:
+ * k_out, v_out [n_rows][kv_heads][head_dim] (with q_off = the prefix sums of
+ * kv_len: whole sequences).  Empty rows give zeros. */
+int rc_kv_read(rc_kv *kv, int layer, int n_rows, const int32_t *table_dev, int cols, int ld_table,
+               const int32_t *kv_len_dev, const int32_t *q_off_dev, int n_seqs, uint16_t *k_out_dev,
+               uint16_t *v_out_dev, void *stream);
+
+/* Copy pages src[i] -> dst[i] (device arrays of n ids) in every layer and,
+ * when table_dev is given, replace every entry src[i] of table
+ * [rows][ld_table] (the first ``cols`` entries of each row) by dst[i], in
+ * one launch.  No page may be both a source and a destination, nor twice a
+ * destination; with a table no page twice a source. */
+int rc_kv_move_pages(rc_kv *kv, const int32_t *src_dev, const int32_t *dst_dev, int n, int32_t *table_dev, int rows,
+                     int cols, int ld_table, void *stream);
+
+/* The pages of a pool as sequences own them (host memory only; no GPU): a
+ * sequence is a list of pages and a token count, a page may belong to several
+ * sequences (forks share it) and is free again when the last one lets it go.
+ * The calls return the page copies that the caller has to launch
+ * (rc_kv_move_pages) before it writes to the sequence.  Calls on one pool are
+ * not thread-safe. */
+typedef struct rc_pages rc_pages;
+int rc_pages_create(int pages, int page_size, rc_pages **out);
+int rc_pages_destroy(rc_pages *p);
+/* A new sequence without tokens. */
+int rc_pages_new(rc_pages *p, int *seq);
+/* counts[i] more tokens for sequence seqs[i], i < n, each listed once.  A
+ * sequence whose last page is partly filled and shared gets a page of its
+ * own: src[j] is to be copied to dst[j] for j < *n_copies (arrays of n).
+ * RC_ERR_FULL, and no change, when too few pages are free for all of them. */
+int rc_pages_extend(rc_pages *p, const int32_t *seqs, const int32_t *counts, int n, int32_t *src, int32_t *dst,
+                    int *n_copies);
+/* A second sequence with the same tokens, sharing every page. */
+int rc_pages_fork(rc_pages *p, int seq, int *child);
+/* Keep the first n tokens. */
+int rc_pages_trim(rc_pages *p, int seq, int n);
+int rc_pages_free(rc_pages *p, int seq);
+/* Move the pages in use to the lowest ids: src[i] -> dst[i] for i < *n
+ * (arrays of at least the pool's page count); the sequences are updated. */
+int rc_pages_compact(rc_pages *p, int32_t *src, int32_t *dst, int *n);
+/* Pages in no sequence, and one past the highest page in use. */
+int rc_pages_info(const rc_pages *p, int *free_pages, int *high_water);
+int rc_pages_len(const rc_pages *p, int seq, int *tokens);
+/* The batch description of n sequences: table [n][ld] (-1 past a sequence's
+ * pages) and kv_len [n], host memory. */
+int rc_pages_table(const rc_pages *p, const int32_t *seqs, int n, int32_t *table, int ld, int32_t *kv_len);
 
 /* rc_gemv without any device allocation (this entry point has no counterpart
  * in the reference).  Arguments and results are those of rc_gemv, bit for

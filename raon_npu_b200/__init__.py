@@ -9,7 +9,7 @@ backend without the built library raises ``RaonCudaError``.
 
 from ._lib import RaonCudaError, DeviceTimeout, load  # noqa: F401
 
-__all__ = ["RaonCudaError", "DeviceTimeout", "load", "CudaBackend", "Context", "Q4nxWeight"]
+__all__ = ["RaonCudaError", "DeviceTimeout", "load", "CudaBackend", "Context", "Q4nxWeight", "KvCache", "KvBatch"]
 
 
 def __getattr__(name):
@@ -19,4 +19,7 @@ def __getattr__(name):
     if name in ("Context", "Q4nxWeight"):
         from . import device
         return getattr(device, name)
+    if name in ("KvCache", "KvBatch"):
+        from . import kvcache
+        return getattr(kvcache, name)
     raise AttributeError(name)

@@ -16,7 +16,7 @@ PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libraon_cuda.so"
 HEADER = PKG.parent / "include" / "raon_cuda.h"
 
-RC_OK, RC_ERR_INVALID, RC_ERR_NOT_FOUND, RC_ERR_CUDA, RC_ERR_TIMEOUT = 0, 1, 2, 3, 4
+RC_OK, RC_ERR_INVALID, RC_ERR_NOT_FOUND, RC_ERR_CUDA, RC_ERR_TIMEOUT, RC_ERR_FULL = 0, 1, 2, 3, 4, 5
 RC_DTYPE_BF16, RC_DTYPE_F32 = 0, 1
 RC_ACT_SWIGLU, RC_ACT_SITU = 0, 1
 RC_ROUTER_SOFTMAX, RC_ROUTER_SIGMOID_BIAS = 0, 1
@@ -31,6 +31,10 @@ class RaonCudaError(RuntimeError):
 
 class DeviceTimeout(RaonCudaError):
     """A kernel's bounded wait gave up and reported it through the error word."""
+
+
+class CacheFull(RaonCudaError):
+    """A KV page pool has too few free pages for a call; nothing was changed."""
 
 
 _P = ctypes.c_void_p
@@ -87,6 +91,24 @@ SIGNATURES = {
     "rc_moe_prefill_combine": (_I, [_P, _P, _P, _I, _I, _I, _P, _P]),
     "rc_sample_tokens": (_I, [_P, _P, _I, _I, _I, _I, _D, _D, _D, _P, _P, _P, _P, _P]),
     "rc_add_bf16": (_I, [_P, _P, _P, _P, ctypes.c_longlong, _P]),
+    "rc_kv_pool_bytes": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(_SZ)]),
+    "rc_kv_create": (_I, [_P, _I, _I, _I, _I, _I, _P, _SZ, ctypes.POINTER(_P)]),
+    "rc_kv_destroy": (_I, [_P]),
+    "rc_kv_append": (_I, [_P, _I, _P, _I, _I, _I, _I, _P, _I, _I, _P, _P, _I, _P, _P, _F, _P, _I, _I, _I, _P, _I, _P]),
+    "rc_kv_attend": (_I, [_P, _I, _P, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _F, _I, _I, _P, _I, _P]),
+    "rc_kv_read": (_I, [_P, _I, _I, _P, _I, _I, _P, _P, _I, _P, _P, _P]),
+    "rc_kv_move_pages": (_I, [_P, _P, _P, _I, _P, _I, _I, _I, _P]),
+    "rc_pages_create": (_I, [_I, _I, ctypes.POINTER(_P)]),
+    "rc_pages_destroy": (_I, [_P]),
+    "rc_pages_new": (_I, [_P, ctypes.POINTER(_I)]),
+    "rc_pages_extend": (_I, [_P, _P, _P, _I, _P, _P, ctypes.POINTER(_I)]),
+    "rc_pages_fork": (_I, [_P, _I, ctypes.POINTER(_I)]),
+    "rc_pages_trim": (_I, [_P, _I, _I]),
+    "rc_pages_free": (_I, [_P, _I]),
+    "rc_pages_compact": (_I, [_P, _P, _P, ctypes.POINTER(_I)]),
+    "rc_pages_info": (_I, [_P, ctypes.POINTER(_I), ctypes.POINTER(_I)]),
+    "rc_pages_len": (_I, [_P, _I, ctypes.POINTER(_I)]),
+    "rc_pages_table": (_I, [_P, _P, _I, _P, _I, _P]),
     "rc_add_rms_bf16": (_I, [_P, _P, _P, _P, _I, _I, _F, _P]),
 }
 
@@ -134,6 +156,8 @@ def check(status: int, what: str = "") -> None:
         raise ValueError(msg)
     if status == RC_ERR_NOT_FOUND:
         raise KeyError(msg)
+    if status == RC_ERR_FULL:
+        raise CacheFull(msg)
     if status == RC_ERR_TIMEOUT:
         raise DeviceTimeout(msg)
     raise RaonCudaError(msg)

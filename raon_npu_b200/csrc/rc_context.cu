@@ -88,6 +88,15 @@ int report_error_word(rc_ctx *ctx, int word) {
       set_error("sampler: the logits have no orderable value (NaN) (device error word 3)");
       return RC_ERR_INVALID;
     }
+    if (word == kErrKvRange) {
+      set_error("KV cache: a page id, length or position outside the cache, its table or the rope table reached the "
+                "device (device error word 5)");
+      return RC_ERR_INVALID;
+    }
+    if (word == kErrKvNonFinite) {
+      set_error("KV cache: a key or value group with a non-finite value was stored as NaN (device error word 6)");
+      return RC_ERR_INVALID;
+    }
     ++ctx->timeout_epoch;
     set_error("a kernel gave up a bounded wait (device error word %d)", word);
     return RC_ERR_TIMEOUT;
@@ -104,6 +113,28 @@ int check_error_word(rc_ctx *ctx) {
 
 int ensure_sample_scratch(rc_ctx *ctx, size_t bytes) {
   return grow_device(&ctx->sample_bits, &ctx->sample_bits_cap, bytes);
+}
+
+// Scratch of one attention call: grows only, after the whole device is idle.
+int ensure_attn_scratch(rc_ctx *ctx, size_t bytes, size_t counters) {
+  if (bytes > ctx->attn_part_cap) {
+    RC_CUDA_TRY(cudaDeviceSynchronize());
+    int rc = grow_device(&ctx->attn_part, &ctx->attn_part_cap, bytes);
+    if (rc) return rc;
+  }
+  if (counters > ctx->attn_count_cap) {
+    RC_CUDA_TRY(cudaDeviceSynchronize());
+    int *c = nullptr;
+    RC_CUDA_TRY(cudaMalloc(&c, counters * sizeof(int)));
+    cudaError_t e = cudaMemset(c, 0, counters * sizeof(int));
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();   // the launch may go to a stream that does not wait for this one
+    if (e != cudaSuccess) cudaFree(c);
+    RC_CUDA_TRY(e);
+    if (ctx->attn_count) cudaFree(ctx->attn_count);
+    ctx->attn_count = c;
+    ctx->attn_count_cap = counters;
+  }
+  return RC_OK;
 }
 
 int ensure_host_staging(rc_ctx *ctx, size_t xb, size_t yb) {
@@ -179,6 +210,8 @@ int rc_destroy(rc_ctx *ctx) {
   cudaFree(ctx->dev_x);
   cudaFree(ctx->dev_y);
   cudaFree(ctx->sample_bits);
+  cudaFree(ctx->attn_part);
+  cudaFree(ctx->attn_count);
   if (ctx->pin_x) cudaFreeHost(ctx->pin_x);
   if (ctx->pin_y) cudaFreeHost(ctx->pin_y);
   if (ctx->pin_err) cudaFreeHost(ctx->pin_err);

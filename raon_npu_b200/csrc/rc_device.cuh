@@ -20,6 +20,34 @@ __device__ __forceinline__ float bf16_to_f32(uint32_t bits16) { return __uint_as
 
 __device__ __forceinline__ float bf16_round(float f) { return bf16_to_f32(f32_to_bf16_rne(f)); }
 
+// bf16 directed rounding of an f32 value (quant/q4nx.py:57-106 on f32 input).
+__device__ __forceinline__ float bf16_floor_f32(float f) {
+  const uint32_t u = __float_as_uint(f);
+  const uint32_t step = ((u >> 31) && (u & 0xFFFFu)) ? 1u : 0u;
+  return __uint_as_float(((u >> 16) + step) << 16);
+}
+__device__ __forceinline__ float bf16_ceil_f32(float f) {
+  const uint32_t u = __float_as_uint(f);
+  const uint32_t step = (!(u >> 31) && (u & 0xFFFFu)) ? 1u : 0u;
+  return __uint_as_float(((u >> 16) + step) << 16);
+}
+// f64 -> nearest f32 not below x, then bf16 ceiling (the f64 branch of bf16_ceil).
+__device__ __forceinline__ float bf16_ceil_f64(double x) {
+  float f = __double2float_rn(x);
+  if ((double)f < x) f = nextafterf(f, INFINITY);
+  return bf16_ceil_f32(f);
+}
+// Next bf16 toward +inf of an exact bf16 value, -0 treated as +0 (quant/q4nx.py:109-124).
+__device__ __forceinline__ float bf16_next_up(float f) {
+  uint32_t t = __float_as_uint(f) >> 16;
+  if (t == 0x8000u) t = 0;
+  uint32_t nxt;
+  if (t == 0) nxt = 1;
+  else if (t & 0x8000u) nxt = (t == 0x8001u) ? 0 : t - 1;
+  else nxt = t + 1;
+  return __uint_as_float(nxt << 16);
+}
+
 __device__ __forceinline__ uint32_t smem_addr(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

@@ -52,6 +52,8 @@ constexpr int kXSlots = 4;
 // Device error words (ctx->err): first failure wins.
 constexpr int kErrWaitTimeout = 1;
 constexpr int kErrBadExpert = 4;       // an expert id outside 0..E-1 reached the device
+constexpr int kErrKvRange = 5;         // a page id, length or position outside the KV cache, table or rope table
+constexpr int kErrKvNonFinite = 6;     // a key or value group with no 4-bit form (NaN, Inf or overflow)
 
 void set_error(const char *fmt, ...);
 
@@ -115,12 +117,18 @@ struct rc_ctx {
   // Sampler scratch: seen-token bitmaps.
   void *sample_bits;
   size_t sample_bits_cap;
+  // Attention scratch: chunk partials and, zero between launches, arrival counters.
+  void *attn_part;
+  size_t attn_part_cap;
+  int *attn_count;
+  size_t attn_count_cap;
 };
 
 namespace rc {
 int ensure_gemv_scratch(rc_ctx *ctx, int k, int n_tiles);
 int ensure_host_staging(rc_ctx *ctx, size_t xb, size_t yb);
 int ensure_sample_scratch(rc_ctx *ctx, size_t bytes);
+int ensure_attn_scratch(rc_ctx *ctx, size_t bytes, size_t counters);
 int check_error_word(rc_ctx *ctx);
 int report_error_word(rc_ctx *ctx, int word);
 // Host staging of the host-buffer entry points (elementwise.cu): pinned host
