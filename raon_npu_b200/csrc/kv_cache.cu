@@ -34,19 +34,19 @@ __device__ __forceinline__ void load_lane(const void *x, size_t at, float (&v)[E
   if constexpr (F32) {
     const float *p = static_cast<const float *>(x) + at;
     if constexpr (E == 4) {
-      const float4 w = *reinterpret_cast<const float4 *>(p);
+      const float4 w = __ldcg(reinterpret_cast<const float4 *>(p));
       v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
     } else {
-      const float2 w = *reinterpret_cast<const float2 *>(p);
+      const float2 w = __ldcg(reinterpret_cast<const float2 *>(p));
       v[0] = w.x, v[1] = w.y;
     }
   } else {
     const uint16_t *p = static_cast<const uint16_t *>(x) + at;
     if constexpr (E == 4) {
-      const uint2 w = *reinterpret_cast<const uint2 *>(p);
+      const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(p));
       v[0] = bf16_lo_f32(w.x), v[1] = bf16_hi_f32(w.x), v[2] = bf16_lo_f32(w.y), v[3] = bf16_hi_f32(w.y);
     } else {
-      const uint32_t w = *reinterpret_cast<const uint32_t *>(p);
+      const uint32_t w = __ldcg(reinterpret_cast<const uint32_t *>(p));
       v[0] = bf16_lo_f32(w), v[1] = bf16_hi_f32(w);
     }
   }
@@ -219,11 +219,12 @@ __global__ void __launch_bounds__(32 * kKvWarps)
     for (int i = 0; i < E / 2; ++i) w[i] = 0;
     if (blk) {
       const uint8_t *codes = blk + (kv ? g.vc_off : 0) + (size_t)t * (D / 2) + (kv ? kv_v_byte(d0, NJ) : kv_k_byte(d0, NJ));
-      const uint32_t par = reinterpret_cast<const uint32_t *>(blk + (kv ? g.vp_off : g.kp_off))[t * NJ + d0 / kKvGroup];
+      const uint32_t par = __ldcg(reinterpret_cast<const uint32_t *>(blk + (kv ? g.vp_off : g.kp_off)) + t * NJ + d0 / kKvGroup);
       const float sc = bf16_lo_f32(par), mn = bf16_hi_f32(par);
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) {
-        const float a = fmaf(sc, (float)(codes[i] & 15), mn), c = fmaf(sc, (float)(codes[i] >> 4), mn);
+        const uint32_t byte = __ldcg(codes + i);
+        const float a = fmaf(sc, (float)(byte & 15), mn), c = fmaf(sc, (float)(byte >> 4), mn);
         w[i] = f32_to_bf16_rne(a) | ((uint32_t)f32_to_bf16_rne(c) << 16);
       }
     }
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(kMoveThreads) rc_kv_move_kernel(const __grid_c
   const int copies = p.n * p.chunks;
   if ((int)blockIdx.x < copies) {
     const int m = blockIdx.x / p.chunks, c = blockIdx.x % p.chunks;
-    const int src = __ldg(p.src + m), dst = __ldg(p.dst + m);
+    const int src = __ldcg(p.src + m), dst = __ldcg(p.dst + m);
     if ((unsigned)src >= (unsigned)p.pages || (unsigned)dst >= (unsigned)p.pages) {
       if (threadIdx.x == 0) atomicCAS(p.err, 0, kErrKvRange);
       return;
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(kMoveThreads) rc_kv_move_kernel(const __grid_c
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int k = threadIdx.x + i * kMoveThreads;
-      if (k < n16) v[i] = __ldcs(a + k);
+      if (k < n16) v[i] = __ldcg(a + k);
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kMoveThreads) rc_kv_move_kernel(const __grid_c
     for (int i = threadIdx.x; i < kMoveSlots; i += kMoveThreads) keys[i] = -1;
     __syncthreads();
     for (int m = m0 + threadIdx.x; m < p.n && m < m0 + kMoveHash; m += kMoveThreads) {
-      const int src = __ldg(p.src + m), dst = __ldg(p.dst + m);
+      const int src = __ldcg(p.src + m), dst = __ldcg(p.dst + m);
       if ((unsigned)src >= (unsigned)p.pages || (unsigned)dst >= (unsigned)p.pages) continue;
       uint32_t s = move_slot(src);
       while (atomicCAS(keys + s, -1, src) != -1) s = (s + 1) % kMoveSlots;   // at most half full
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(kMoveThreads) rc_kv_move_kernel(const __grid_c
     __syncthreads();
     for (int i = threadIdx.x; i < kMoveEntries && e0 + i < total; i += kMoveThreads) {
       int32_t *e = p.table + (e0 + i) / p.cols * p.ld + (e0 + i) % p.cols;
-      const int id = *e;
+      const int id = __ldcg(e);
       if (id < 0) continue;
       for (uint32_t s = move_slot(id); keys[s] != -1; s = (s + 1) % kMoveSlots)
         if (keys[s] == id) {

@@ -18,6 +18,11 @@ namespace rc {
 constexpr int kKvGroup = 32;        // values per (scale, min)
 constexpr int kKvMaxSeqs = 4096;    // sequences of one batch
 
+// The calls of a step are chained by programmatic dependent launch, so a
+// neighbour's CTA may have filled this SM's L1 with lines that the previous
+// call rewrote: whatever earlier calls write (tables, lengths, queries, the
+// cache) is read past L1 (ld.cg, bulk copies).
+
 // One layer of a pool.  A head block: K codes, K params, V codes, V params.
 struct KvGeom {
   uint8_t *base;
@@ -59,20 +64,20 @@ __device__ __forceinline__ bool kv_find_row(const KvBatchDev &b, int r, int lane
   if (!b.q_off) {
     if (r >= b.n_seqs) return false;
     seq = r;
-    pos = __ldg(b.kv_len + r) - 1;
+    pos = __ldcg(b.kv_len + r) - 1;
     return true;
   }
   int below = 0;   // offsets <= r
   for (int k0 = 0; k0 <= b.n_seqs; k0 += 32) {
     const int k = k0 + lane;
-    const unsigned m = __ballot_sync(0xffffffffu, k <= b.n_seqs && __ldg(b.q_off + k) <= r);
+    const unsigned m = __ballot_sync(0xffffffffu, k <= b.n_seqs && __ldcg(b.q_off + k) <= r);
     below += __popc(m);
     if (m != 0xffffffffu) break;
   }
   seq = below - 1;
   if (seq < 0 || seq >= b.n_seqs) return false;
-  const int lo = __ldg(b.q_off + seq), hi = __ldg(b.q_off + seq + 1);
-  pos = __ldg(b.kv_len + seq) - (hi - lo) + (r - lo);
+  const int lo = __ldcg(b.q_off + seq), hi = __ldcg(b.q_off + seq + 1);
+  pos = __ldcg(b.kv_len + seq) - (hi - lo) + (r - lo);
   return true;
 }
 
@@ -81,7 +86,7 @@ __device__ __forceinline__ bool kv_find_row(const KvBatchDev &b, int r, int lane
 __device__ __forceinline__ uint8_t *kv_head_block(const KvGeom &g, const KvBatchDev &b, int seq, int pos, int head,
                                                   int *err) {
   const int pi = pos >> g.log2_page;
-  const int id = pi < b.cols ? __ldg(b.table + (size_t)seq * b.ld + pi) : -1;
+  const int id = pi < b.cols ? __ldcg(b.table + (size_t)seq * b.ld + pi) : -1;
   if (id < 0 || id >= g.pages) {
     atomicCAS(err, 0, kErrKvRange);
     return nullptr;
