@@ -41,18 +41,21 @@ namespace rc {
 constexpr int kDcWarps = 4;                       // computing warps
 constexpr int kDcThreads = 32 * (kDcWarps + 1);   // and one that copies
 constexpr int kDcStage = 64;                      // tokens of a stage
-constexpr int kDcChunk = 256;                     // smallest chunk
+constexpr int kDcChunk = 256;                     // smallest chunk ...
+constexpr int kDcMaxChunk = 1024;                 // ... and the largest that more than 16 of a length are cut for
 constexpr int kDcMaxChunks = 128;                 // chunks of a visible length ...
 constexpr int kDcChunkSlots = kDcMaxChunks + 3;   // ... and those a window and sinks cut at their ends
+constexpr int kDcFan = 16;                        // partial results joined at a time
+constexpr int kDcGroups = (kDcChunkSlots + kDcFan - 1) / kDcFan;
 constexpr float kDcSlack = 8.f;                   // how far a score may pass the softmax reference, log2
 constexpr float kDcLift = 7.f;                    // weights are 2^(score - reference + lift): at most 2^15
 
 struct DcParams {
   AttnParams a;
   int cbs;            // column blocks of max_q rows
-  int slots;          // partials of one (sequence, head, column block)
+  int slots;          // partials of one (sequence, head, column block): its chunks', then its groups'
   float *part;        // [n_seqs][heads][cbs][slots][cols * (D + 2)]
-  int *count;         // [n_seqs][heads][cbs]
+  int *count;         // [n_seqs][heads][cbs][1 + groups] arrivals, zero between launches
 };
 
 // What a sequence's items need.
@@ -69,6 +72,7 @@ __device__ __forceinline__ DcSeq dc_seq(const AttnParams &p, int b) {
   s.sinks = p.window > 0 ? min(p.sinks, s.lo) : 0;
   const int span = s.len - s.lo + s.sinks;
   s.chunk = kDcChunk;
+  while (s.chunk < kDcMaxChunk && span > 16 * s.chunk) s.chunk *= 2;
   while (s.chunk < span / kDcMaxChunks + (span % kDcMaxChunks != 0)) s.chunk *= 2;
   s.c_lo = s.lo / s.chunk;
   s.n_sink = min((s.sinks + s.chunk - 1) / s.chunk, s.c_lo);
@@ -164,10 +168,9 @@ struct DcLayout {
   static constexpr int stage = kDcStage * D * 5 / 4;
   static constexpr int stages = NJ == 4 ? (NB == 1 ? 5 : 7) : (NB == 1 ? 8 : 12);
   static constexpr int join = kDcWarps * cols * D * 4;                       // the warps' values of one item
-  static constexpr int ml = cols * kDcChunkSlots * 8;                        // (maximum, sum) of a row's chunks
-  static constexpr int scratch = join > ml ? join : ml;
+  static_assert(join >= cols * kDcFan * 8, "the joined parts' (reference, sum) lie there too");
   static constexpr int o_scratch = stages * stage;
-  static constexpr int o_vpar = o_scratch + scratch;                         // [warps][8 token pairs][NJ]{scale, min} f16x2
+  static constexpr int o_vpar = o_scratch + join;                         // [warps][8 token pairs][NJ]{scale, min} f16x2
   static constexpr int vpar = 8 * NJ * 8;
   static constexpr int o_ml = o_vpar + kDcWarps * vpar;                      // [2][warps][cols]
   static constexpr int o_bar = o_ml + 2 * kDcWarps * cols * 4;
@@ -175,6 +178,54 @@ struct DcLayout {
   static constexpr int o_prefix = o_flags + 16;
   static int bytes(int n_seqs) { return o_prefix + (n_seqs + 1) * 4; }
 };
+
+// The CTA's writes are out; true in every thread of the CTA that arrives last
+// of n, which then sees the others' writes (and finds the counter at zero again).
+__device__ __forceinline__ bool dc_arrive_last(int *count, int n, volatile int *s_last, int tid) {
+  __threadfence();
+  dc_sync();
+  if (tid == 0) {
+    const bool last = atomicAdd(count, 1) == n - 1;
+    *s_last = last;
+    if (last) *count = 0;
+  }
+  dc_sync();
+  if (!*s_last) return false;
+  __threadfence();
+  return true;
+}
+
+// Joins n <= kDcFan partial results in order; sink(column, value, 4 sums, reference, sum).
+template <int NJ, int NB, typename Sink>
+__device__ __forceinline__ void dc_join(const float *src, int n, float *scratch, int tid, Sink sink) {
+  constexpr int D = 32 * NJ, NC = 8 * NB;
+  constexpr size_t kSlot = (size_t)NC * (D + 2);
+  float2 *ml = reinterpret_cast<float2 *>(scratch);   // [part][column]
+  dc_sync();
+  for (int e = tid; e < n * NC; e += 32 * kDcWarps)
+    ml[e] = __ldcg(reinterpret_cast<const float2 *>(src + (e / NC) * kSlot + (size_t)NC * D) + e % NC);
+  dc_sync();
+#pragma unroll 1
+  for (int e = tid; e < NC * D / 4; e += 32 * kDcWarps) {
+    const int col = e / (D / 4), d = 4 * (e % (D / 4));
+    float4 v[kDcFan];
+#pragma unroll
+    for (int c = 0; c < kDcFan; ++c)
+      v[c] = c < n ? __ldcg(reinterpret_cast<const float4 *>(src + c * kSlot + (size_t)col * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, sum = 0.f;
+    for (int c = 0; c < n; ++c) top = fmaxf(top, ml[c * NC + col].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < kDcFan; ++c) {
+      if (c >= n) break;
+      const float2 x = ml[c * NC + col];
+      const float f = top == -INFINITY ? 1.f : exp2f(x.x - top);
+      sum = fmaf(f, x.y, sum);
+      acc.x = fmaf(f, v[c].x, acc.x), acc.y = fmaf(f, v[c].y, acc.y), acc.z = fmaf(f, v[c].z, acc.z), acc.w = fmaf(f, v[c].w, acc.w);
+    }
+    sink(col, d, acc, top, sum);
+  }
+}
 
 // MULTI: the rows of a sequence have masks of their own.
 template <int NJ, int NB, bool MULTI>
@@ -623,46 +674,28 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
       }
     }
     if (s.n_chunks > 1) {
-      __threadfence();
-      dc_sync();
-      if (tid == 0) {
-        const int before = atomicAdd(p.count + cell, 1);
-        *s_last = before == s.n_chunks - 1;
-        if (*s_last) p.count[cell] = 0;
-      }
-      dc_sync();
-      if (*s_last) {
-        __threadfence();
-        float2 *ml = reinterpret_cast<float2 *>(s_o);     // [chunk][column]; the shares are done with
-        const float *src = p.part + cell * p.slots * kSlot;
-        for (int e = tid; e < s.n_chunks * NC; e += 32 * kDcWarps)
-          ml[e] = __ldcg(reinterpret_cast<const float2 *>(src + (e / NC) * kSlot + (size_t)NC * D) + e % NC);
-        dc_sync();
-        for (int col = warp; col < NC; col += kDcWarps) {
-          float top = -INFINITY, sum = 0.f;
-          for (int c = lane; c < s.n_chunks; c += 32) top = fmaxf(top, ml[c * NC + col].x);
-#pragma unroll
-          for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-          for (int c = lane; c < s.n_chunks; c += 32) {
-            const float f = top == -INFINITY ? 1.f : exp2f(ml[c * NC + col].x - top);
-            sum = fmaf(f, ml[c * NC + col].y, sum);
-            ml[c * NC + col].x = f;
-          }
-#pragma unroll
-          for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-          if (lane == 0) s_l[col] = sum;
-        }
-        dc_sync();
-        for (int e = tid; e < NC * D / 4; e += 32 * kDcWarps) {
-          const int col = e / (D / 4), d = 4 * (e % (D / 4));
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int c = 0; c < s.n_chunks; ++c) {
-            const float f = ml[c * NC + col].x;
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(src + c * kSlot + (size_t)col * D + d));
-            acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
-          }
-          attn_write4(a, s.first, s.rows_do, it.cb * NC + col, it.head, D, d, acc, s_l[col]);
+      // the last chunk of a group joins the group, the last group's joiner the row; always in order
+      float *cell_part = p.part + cell * p.slots * kSlot;
+      int *count = p.count + cell * (kDcGroups + 1);
+      const int groups = (s.n_chunks + kDcFan - 1) / kDcFan, grp = it.chunk / kDcFan;
+      if (dc_arrive_last(count + 1 + grp, min(kDcFan, s.n_chunks - grp * kDcFan), s_last, tid)) {
+        const float *src = cell_part + (size_t)grp * kDcFan * kSlot;
+        const int n = min(kDcFan, s.n_chunks - grp * kDcFan);
+        if (groups == 1) {
+          dc_join<NJ, NB>(src, n, s_o, tid, [&](int col, int d, float4 acc, float top, float sum) {
+            attn_write4(a, s.first, s.rows_do, it.cb * NC + col, it.head, D, d, acc, sum);
+          });
+        } else {
+          float *mid = cell_part + (size_t)(p.slots - kDcGroups) * kSlot;
+          dc_join<NJ, NB>(src, n, s_o, tid, [&](int col, int d, float4 acc, float top, float sum) {
+            float *dst = mid + grp * kSlot;
+            __stcg(reinterpret_cast<float4 *>(dst + (size_t)col * D + d), acc);
+            if (d == 0) __stcg(reinterpret_cast<float2 *>(dst + (size_t)NC * D + 2 * col), make_float2(top, sum));
+          });
+          if (dc_arrive_last(count, groups, s_last, tid))
+            dc_join<NJ, NB>(mid, groups, s_o, tid, [&](int col, int d, float4 acc, float top, float sum) {
+              attn_write4(a, s.first, s.rows_do, it.cb * NC + col, it.head, D, d, acc, sum);
+            });
         }
       }
     }
@@ -676,10 +709,10 @@ static int decode_launch(rc_ctx *ctx, DcParams &p, int max_q, cudaStream_t s) {
   const AttnParams &a = p.a;
   const long long max_len = (long long)a.b.cols * a.g.page, chunks = (max_len + kDcChunk - 1) / kDcChunk;
   p.cbs = (int)(((long long)max_q * a.group + L::cols - 1) / L::cols);
-  p.slots = (int)(chunks < kDcChunkSlots ? chunks : kDcChunkSlots);
+  p.slots = (int)(chunks < kDcChunkSlots ? chunks : kDcChunkSlots) + kDcGroups;
   const long long cells = (long long)a.b.n_seqs * a.g.heads * p.cbs;
   RC_CHECK_ARG(cells * p.slots <= INT_MAX, "rc_kv_attend: the batch is too large");
-  int rc = ensure_attn_scratch(ctx, (size_t)cells * p.slots * L::cols * (L::D + 2) * sizeof(float), (size_t)cells);
+  int rc = ensure_attn_scratch(ctx, (size_t)cells * p.slots * L::cols * (L::D + 2) * sizeof(float), (size_t)cells * (kDcGroups + 1));
   if (rc) return rc;
   p.part = static_cast<float *>(ctx->attn_part);
   p.count = ctx->attn_count;
