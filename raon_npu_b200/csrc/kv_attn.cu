@@ -3,6 +3,9 @@
 
 using namespace rc;
 
+// Rows of a sequence and kv head above which a call goes to the tensor-core kernel.
+constexpr long long kPromptRows = 255;
+
 extern "C" int rc_kv_attend(rc_kv *kv, int layer, const uint16_t *q_dev, int ldq, int q_heads, int n_rows,
                             const int32_t *table_dev, int cols, int ld_table,
                             const int32_t *kv_len_dev, const int32_t *q_off_dev, int n_seqs, int max_q, float scale, int window, int sinks,
@@ -34,5 +37,6 @@ extern "C" int rc_kv_attend(rc_kv *kv, int layer, const uint16_t *q_dev, int ldq
   p.out = out_dev;
   p.ldo = ldo;
   p.err = kv->ctx->err;
-  return kv_attend_decode(kv->ctx, p, p.max_q, pick_stream(kv->ctx, stream));
+  const cudaStream_t s = pick_stream(kv->ctx, stream);
+  return (long long)p.max_q * p.group > kPromptRows ? kv_attend_prompt(kv->ctx, p, s) : kv_attend_decode(kv->ctx, p, p.max_q, s);
 }

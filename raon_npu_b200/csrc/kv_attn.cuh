@@ -1,10 +1,32 @@
 // What the attention kernels over the 4-bit KV cache share.
 #pragma once
 
+#include <atomic>
+
 #include "kv_internal.cuh"
 
 namespace rc {
 
+constexpr float kAttnSlack = 8.f;   // how far a score may pass a row's softmax reference, log2
+constexpr float kAttnLift = 7.f;    // weights are 2^(score - reference + lift): at most 2^15
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+// a * b + c in f16, one rounding; subnormal operands are exact.
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// 2^x to 2 ulp of 32 bits; results below 2^-126 are zero.
+__device__ __forceinline__ float ex2(float x) {
+  float d;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
+  return d;
+}
 struct AttnParams {
   KvGeom g;
   KvBatchDev b;
@@ -53,5 +75,6 @@ __device__ __forceinline__ void attn_write4(const AttnParams &p, int first, int 
 }
 
 int kv_attend_decode(rc_ctx *ctx, const AttnParams &a, int max_q, cudaStream_t s);   // kv_decode.cu
+int kv_attend_prompt(rc_ctx *ctx, const AttnParams &a, cudaStream_t s);              // kv_prompt.cu
 
 }  // namespace rc

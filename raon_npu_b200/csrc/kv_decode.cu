@@ -32,8 +32,6 @@
 // arrive joins them in chunk order.
 #include <limits.h>
 
-#include <atomic>
-
 #include "kv_attn.cuh"
 
 namespace rc {
@@ -47,8 +45,6 @@ constexpr int kDcMaxChunks = 128;                 // chunks of a visible length 
 constexpr int kDcChunkSlots = kDcMaxChunks + 3;   // ... and those a window and sinks cut at their ends
 constexpr int kDcFan = 16;                        // partial results joined at a time
 constexpr int kDcGroups = (kDcChunkSlots + kDcFan - 1) / kDcFan;
-constexpr float kDcSlack = 8.f;                   // how far a score may pass the softmax reference, log2
-constexpr float kDcLift = 7.f;                    // weights are 2^(score - reference + lift): at most 2^15
 
 struct DcParams {
   AttnParams a;
@@ -118,23 +114,6 @@ __device__ __forceinline__ int dc_chunk_start(const DcSeq &s, int i) {
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-  return d;
-}
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-// a * b + c in f16, one rounding; subnormal operands are exact.
-__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-// 2^x to 2 ulp of 32 bits; results below 2^-126 are zero.
-__device__ __forceinline__ float ex2(float x) {
-  float d;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
   return d;
 }
 __device__ __forceinline__ void dc_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kDcWarps) : "memory"); }
@@ -474,7 +453,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) over = over || fmaxf(x[nb][0][c], x[nb][1][c]) > m[nb][c] + kDcSlack;
+          for (int c = 0; c < 2; ++c) over = over || fmaxf(x[nb][0][c], x[nb][1][c]) > m[nb][c] + kAttnSlack;
         // exponents: of the scales, and of minima more than 2^19 times as large
         int ve = 0;
         bool poison = false;
@@ -519,7 +498,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
               float al = 1.f;
-              if (mx > m[nb][c] + kDcSlack) {
+              if (mx > m[nb][c] + kAttnSlack) {
                 al = exp2f(m[nb][c] - mx);
                 m[nb][c] = mx;
               }
@@ -541,7 +520,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float ref = m[nb][c] == -INFINITY ? 0.f : m[nb][c] - kDcLift;
+            const float ref = m[nb][c] == -INFINITY ? 0.f : m[nb][c] - kAttnLift;
             w[nb][0][c] = ex2(x[nb][0][c] - ref);
             w[nb][1][c] = ex2(x[nb][1][c] - ref);
             l[nb][c] += w[nb][0][c] + w[nb][1][c];
