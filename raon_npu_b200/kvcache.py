@@ -21,10 +21,18 @@ from __future__ import annotations
 import ctypes
 
 import numpy as np
+import torch
 
 from . import _lib
 from ._lib import check
-from .device import Context, _ptr, _stream_for
+from .device import CUDA_STREAM_LEGACY, Context, _ptr
+
+# A decode step makes one or two of these calls a layer, so the checks below
+# are written for the host's time: get_device() (-1 on the CPU) instead of
+# device objects, is_contiguous() before strides.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_BF16 = frozenset((torch.bfloat16, torch.int16, torch.uint16))   # bf16 values, or their bits
+_F32 = frozenset((torch.float32,))
 
 
 def rope_table(positions: int, rope_dim: int, base: float = 10000.0) -> np.ndarray:
@@ -36,30 +44,31 @@ def rope_table(positions: int, rope_dim: int, base: float = 10000.0) -> np.ndarr
 
 
 def _ints(t, ndim: int, what: str):
-    if str(t.dtype) != "torch.int32" or t.dim() != ndim or not t.is_cuda or (t.shape[-1] > 1 and t.stride(-1) != 1):
+    if t.dtype is not torch.int32 or t.dim() != ndim or not t.is_cuda or (t.shape[-1] > 1 and t.stride(-1) != 1):
         raise ValueError(f"{what} must be an int32 CUDA tensor of {ndim} dimension(s), contiguous in the last")
     return t
 
 
-def _rows(t, width: int, what: str, size: int = 2):
-    """(rows, row stride in elements) of [rows, width] or [rows, heads, head_dim] values of ``size`` bytes."""
+def _rows(t, width: int, what: str, dev: int, types=_BF16):
+    """(rows, row stride in elements) of [rows, width] or [rows, heads, head_dim] values."""
+    if t.dtype not in types or t.get_device() != dev:
+        raise ValueError(f"{what} must be a {'bf16' if types is _BF16 else 'f32'} tensor on cuda:{dev}, got {t.dtype} on {t.device}")
     shape = t.shape
-    if t.element_size() != size or not t.is_cuda:
-        raise ValueError(f"{what} must be a CUDA tensor of {8 * size}-bit values, got {t.dtype}")
-    if t.dim() == 2:
-        inner = shape[1] == width and (width == 1 or t.stride(1) == 1)
-    elif t.dim() == 3:
-        inner = (shape[1] * shape[2] == width and (shape[2] == 1 or t.stride(2) == 1) and
-                 (shape[1] == 1 or t.stride(1) == shape[2]))
+    if len(shape) == 2:
+        inner = shape[1] == width and (t.is_contiguous() or width == 1 or t.stride(1) == 1)
+    elif len(shape) == 3:
+        inner = shape[1] * shape[2] == width and (t.is_contiguous() or (
+            (shape[2] == 1 or t.stride(2) == 1) and (shape[1] == 1 or t.stride(1) == shape[2])))
     else:
         inner = False
     if not inner:
         raise ValueError(f"{what} must hold rows of {width} contiguous values, got {tuple(shape)} "
                          f"with strides {tuple(t.stride())}")
-    ld = int(t.stride(0)) if shape[0] > 1 else width
+    rows = shape[0]
+    ld = t.stride(0) if rows > 1 else width
     if ld < width:
         raise ValueError(f"{what}: rows overlap (stride {ld} of {width} values)")
-    return int(shape[0]), ld
+    return rows, ld
 
 
 class KvBatch:
@@ -104,6 +113,7 @@ class KvCache:
         self.ctx, self.lib = ctx, ctx.lib
         self.layers, self.kv_heads, self.head_dim = int(layers), int(kv_heads), int(head_dim)
         self.pages, self.page_size = int(pages), int(page_size)
+        self.scale = self.head_dim ** -0.5
         nbytes = 0
         if pool is not None:
             if not pool.is_cuda or not pool.is_contiguous() or pool.device.index != ctx.device:
@@ -139,11 +149,16 @@ class KvCache:
             pass
 
     def _batch_args(self, batch: KvBatch, rows: int, what: str):
-        if batch.table.device.index != self.ctx.device:
+        q_off = batch.q_off
+        if batch.table.get_device() != self.ctx.device:
             raise ValueError(f"{what}: the batch is on {batch.table.device}, the cache on cuda:{self.ctx.device}")
-        if batch.q_off is None and rows != batch.n_seqs:
+        if q_off is None and rows != batch.n_seqs:
             raise ValueError(f"{what}: {rows} rows for {batch.n_seqs} sequences without q_off")
-        return batch.table.data_ptr(), batch.kv_len.data_ptr(), None if batch.q_off is None else batch.q_off.data_ptr()
+        return batch.table.data_ptr(), batch.kv_len.data_ptr(), None if q_off is None else q_off.data_ptr()
+
+    def _stream(self, stream) -> int:
+        """The stream to launch on; torch's default stream is the legacy one (0 is the context's own in the C ABI)."""
+        return int(stream) if stream is not None else _raw_stream(self.ctx.device) or CUDA_STREAM_LEGACY
 
     # ---------------------------------------------------------- operators --
     def append(self, layer: int, x, batch: KvBatch, q_out=None, q_heads: int = 0, q_norm=None, k_norm=None,
@@ -155,30 +170,33 @@ class KvCache:
         the query and key heads (None: no norm).  rope f32 [positions,
         rope_dim]: cos | sin of every position (None: no rotation)."""
         width = (q_heads + 2 * self.kv_heads) * self.head_dim
-        f32 = str(x.dtype) == "torch.float32"
-        rows, ldx = _rows(x, width, "x", 4 if f32 else 2)
+        dev = self.ctx.device
+        f32 = x.dtype is torch.float32
+        rows, ldx = _rows(x, width, "x", dev, _F32 if f32 else _BF16)
         ldq = 0
         if q_heads:
             if q_out is None:
                 raise ValueError("append: q_out is missing")
-            n, ldq = _rows(q_out, q_heads * self.head_dim, "q_out")
+            n, ldq = _rows(q_out, q_heads * self.head_dim, "q_out", dev)
             if n != rows:
                 raise ValueError(f"append: x has {rows} rows, q_out {n}")
         for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-            if w is not None and (w.element_size() != 2 or not w.is_cuda or w.numel() != self.head_dim or
+            if w is not None and (w.dtype not in _BF16 or w.get_device() != dev or w.numel() != self.head_dim or
                                   not w.is_contiguous()):
                 raise ValueError(f"{name} must hold {self.head_dim} bf16 values on the device")
         rope_rows = rope_dim = 0
         if rope is not None:
-            if str(rope.dtype) != "torch.float32" or rope.dim() != 2 or not rope.is_cuda or not rope.is_contiguous():
-                raise ValueError("rope must be a contiguous f32 CUDA tensor [positions, rope_dim]")
-            rope_rows, rope_dim = int(rope.shape[0]), int(rope.shape[1])
+            if rope.dtype is not torch.float32 or rope.dim() != 2 or rope.get_device() != dev or not rope.is_contiguous():
+                raise ValueError(f"rope must be a contiguous f32 tensor [positions, rope_dim] on cuda:{dev}")
+            rope_rows, rope_dim = rope.shape
         table, kv_len, q_off = self._batch_args(batch, rows, "append")
-        check(self.lib.rc_kv_append(
+        rc = self.lib.rc_kv_append(
             self.handle, layer, x.data_ptr(), _lib.RC_DTYPE_F32 if f32 else _lib.RC_DTYPE_BF16, ldx, q_heads, rows,
-            table, batch.columns, batch.ld, kv_len, q_off, batch.n_seqs, _ptr(q_norm) or None, _ptr(k_norm) or None, eps,
-            _ptr(rope) or None, rope_rows, rope_dim, bool(interleaved), _ptr(q_out) or None, ldq,
-            _stream_for(stream, x)), "rc_kv_append")
+            table, batch.columns, batch.ld, kv_len, q_off, batch.n_seqs, None if q_norm is None else q_norm.data_ptr(),
+            None if k_norm is None else k_norm.data_ptr(), eps, None if rope is None else rope.data_ptr(), rope_rows,
+            rope_dim, 1 if interleaved else 0, q_out.data_ptr() if q_heads else None, ldq, self._stream(stream))
+        if rc:
+            check(rc, "rc_kv_append")
 
     def attend(self, layer: int, q, batch: KvBatch, out, scale: float | None = None, window: int = 0, sinks: int = 0,
                stream: int | None = None) -> None:
@@ -187,28 +205,34 @@ class KvCache:
         scale: of the scores (default 1 / sqrt(head_dim)).  window > 0: a row
         sees itself, the window - 1 tokens before it and the first ``sinks``
         tokens of its sequence; 0: every token up to itself."""
-        width = int(q.shape[1]) if q.dim() == 2 else int(q.shape[1]) * int(q.shape[2]) if q.dim() == 3 else 0
+        dev = self.ctx.device
+        shape = q.shape
+        width = shape[1] if len(shape) == 2 else shape[1] * shape[2] if len(shape) == 3 else 0
         heads = width // self.head_dim
-        rows, ldq = _rows(q, heads * self.head_dim, "q")
-        n, ldo = _rows(out, width, "out")
+        rows, ldq = _rows(q, heads * self.head_dim, "q", dev)
+        n, ldo = _rows(out, width, "out", dev)
         if n != rows:
             raise ValueError(f"attend: q has {rows} rows, out {n}")
         table, kv_len, q_off = self._batch_args(batch, rows, "attend")
-        check(self.lib.rc_kv_attend(
-            self.handle, layer, q.data_ptr(), ldq, heads, rows, table, batch.columns, batch.ld, kv_len, q_off, batch.n_seqs,
-            batch.max_q, self.head_dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), ldo,
-            _stream_for(stream, q)), "rc_kv_attend")
+        rc = self.lib.rc_kv_attend(
+            self.handle, layer, q.data_ptr(), ldq, heads, rows, table, batch.columns, batch.ld, kv_len, q_off,
+            batch.n_seqs, batch.max_q, self.scale if scale is None else scale, window, sinks, out.data_ptr(), ldo,
+            self._stream(stream))
+        if rc:
+            check(rc, "rc_kv_attend")
 
     def read(self, layer: int, batch: KvBatch, k_out, v_out, stream: int | None = None) -> None:
         """The cached keys and values of the batch's rows in bf16: k_out, v_out [rows, kv_heads, head_dim], contiguous."""
         width = self.kv_heads * self.head_dim
-        rows, ldk = _rows(k_out, width, "k_out")
-        n, ldv = _rows(v_out, width, "v_out")
+        rows, ldk = _rows(k_out, width, "k_out", self.ctx.device)
+        n, ldv = _rows(v_out, width, "v_out", self.ctx.device)
         if n != rows or ldk != width or ldv != width:
             raise ValueError("read: k_out and v_out must be contiguous and of one shape")
         table, kv_len, q_off = self._batch_args(batch, rows, "read")
-        check(self.lib.rc_kv_read(self.handle, layer, rows, table, batch.columns, batch.ld, kv_len, q_off, batch.n_seqs,
-                                  k_out.data_ptr(), v_out.data_ptr(), _stream_for(stream, k_out)), "rc_kv_read")
+        rc = self.lib.rc_kv_read(self.handle, layer, rows, table, batch.columns, batch.ld, kv_len, q_off, batch.n_seqs,
+                                 k_out.data_ptr(), v_out.data_ptr(), self._stream(stream))
+        if rc:
+            check(rc, "rc_kv_read")
 
     def move_pages(self, src, dst, table=None, stream: int | None = None) -> None:
         """Copy pages src[i] -> dst[i] in every layer and rewrite ``table``'s entries accordingly, in one launch.
@@ -222,11 +246,14 @@ class KvCache:
         rows = cols = ld = 0
         if table is not None:
             _ints(table, 2, "table")
-            rows, cols = int(table.shape[0]), int(table.shape[1])
-            ld = int(table.stride(0)) if rows > 1 else cols
-        check(self.lib.rc_kv_move_pages(self.handle, src.data_ptr(), dst.data_ptr(), int(src.shape[0]),
-                                        _ptr(table) or None, rows, cols, ld, _stream_for(stream, src)),
-              "rc_kv_move_pages")
+            rows, cols = table.shape
+            ld = table.stride(0) if rows > 1 else cols
+        if src.get_device() != self.ctx.device or dst.get_device() != self.ctx.device:
+            raise ValueError(f"move_pages: the moves must be on cuda:{self.ctx.device}")
+        rc = self.lib.rc_kv_move_pages(self.handle, src.data_ptr(), dst.data_ptr(), src.shape[0],
+                                       None if table is None else table.data_ptr(), rows, cols, ld, self._stream(stream))
+        if rc:
+            check(rc, "rc_kv_move_pages")
 
     # ------------------------------------------------------------- pages --
     @property
@@ -266,7 +293,6 @@ class KvCache:
 
     def batch(self, seqs, rows=None, columns: int | None = None) -> KvBatch:
         """Device tables of ``seqs``; rows: how many of each sequence's last tokens are this call's (None: one)."""
-        import torch
         seqs = list(seqs)
         table, kv_len = self.page_pool.table(seqs, columns)
         dev = torch.device("cuda", self.ctx.device)
@@ -281,7 +307,6 @@ class KvCache:
 
     def _move(self, moves, stream) -> None:
         if moves:
-            import torch
             dev = torch.device("cuda", self.ctx.device)
             m = torch.tensor(moves, dtype=torch.int32).t().contiguous().to(dev)
             self.move_pages(m[0], m[1], stream=stream)
