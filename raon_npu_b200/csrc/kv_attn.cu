@@ -16,6 +16,10 @@ extern "C" int rc_kv_attend(rc_kv *kv, int layer, const uint16_t *q_dev, int ldq
   RC_CHECK_ARG(q_heads >= kv->heads && q_heads % kv->heads == 0 && q_heads <= 4096,
                "rc_kv_attend: %d query heads over %d kv heads", q_heads, kv->heads);
   RC_CHECK_ARG(max_q >= 1, "rc_kv_attend: max_q %d", max_q);
+  const int group = q_heads / kv->heads;
+  RC_CHECK_ARG(group <= kAttnMaxGroup && (long long)max_q * group <= kAttnMaxFlat,
+               "rc_kv_attend: %d query heads a kv head (at most %d), %d rows a sequence (rows x heads at most %lld)", group,
+               kAttnMaxGroup, max_q, kAttnMaxFlat);
   RC_CHECK_ARG(ldq >= q_heads * kv->dim && ldo >= q_heads * kv->dim, "rc_kv_attend: rows of %d and %d values, %d are needed",
                ldq, ldo, q_heads * kv->dim);
   RC_CHECK_ARG(ldq % 8 == 0 && ldo % 8 == 0 &&
@@ -29,7 +33,8 @@ extern "C" int rc_kv_attend(rc_kv *kv, int layer, const uint16_t *q_dev, int ldq
   p.b = KvBatchDev{table_dev, kv_len_dev, q_off_dev, cols, ld_table, n_seqs, n_rows};
   p.q = q_dev;
   p.ldq = ldq;
-  p.group = q_heads / kv->heads;
+  p.group = group;
+  p.by_group = make_fastdiv((uint32_t)group);
   p.max_q = q_off_dev ? max_q : 1;
   p.scale_log2 = scale * 1.44269504088896340736f;
   p.window = window;

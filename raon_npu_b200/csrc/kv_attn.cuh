@@ -15,6 +15,11 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
 // a * b + c in f16, one rounding; subnormal operands are exact.
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
@@ -27,11 +32,44 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
   return d;
 }
+// Words from shared memory, in loads of up to 16 bytes.
+template <int N>
+__device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N]) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t *>(p);
+  }
+}
+
+// A warp's wait for a phase of an mbarrier: one verdict for all lanes, false
+// when it gave up (about a second of clock cycles) or another warp had
+// (``abort``), so that every role runs to its end.
+__device__ __forceinline__ bool attn_wait(uint32_t bar, uint32_t parity, volatile int *abort, int *err) {
+  bool there = mbar_try_wait(bar, parity);
+  if (!there) {
+    const uint32_t t0 = (uint32_t)clock();
+    while (!(there = mbar_try_wait(bar, parity))) {
+      if ((uint32_t)clock() - t0 > 2000000000u) {
+        *abort = 1;
+        atomicCAS(err, 0, kErrWaitTimeout);
+      }
+      if (*abort) break;
+    }
+  }
+  return __all_sync(0xffffffffu, there);
+}
+
 struct AttnParams {
   KvGeom g;
   KvBatchDev b;
   const uint16_t *q;
   int ldq, group;        // query heads of a kv head
+  FastDiv by_group;
   int max_q;
   float scale_log2;      // scale * log2(e): scores are in powers of two
   int window, sinks;
@@ -39,6 +77,12 @@ struct AttnParams {
   int ldo;
   int *err;
 };
+
+// Rows of a sequence and kv head are numbered row * group + head in the group;
+// within these limits FastDiv is exact.
+constexpr int kAttnMaxGroup = 256;
+constexpr long long kAttnMaxFlat = 1 << 24;
+__device__ __forceinline__ int attn_row(const AttnParams &p, int flat) { return (int)fdiv((uint32_t)flat, p.by_group); }
 
 // First row, rows and tokens of a sequence; rows_do: the rows that are
 // computed.  Values that do not fit the buffers set the error word and are cut.
@@ -65,10 +109,10 @@ __device__ __forceinline__ void attn_seq(const AttnParams &p, int b, int &first,
 // of a sequence: acc / sum, zeros when nothing was seen.
 __device__ __forceinline__ void attn_write4(const AttnParams &p, int first, int rows_do, int flat, int head, int D, int d,
                                             float4 acc, float sum) {
-  const int qi = flat / p.group;
+  const int qi = attn_row(p, flat);
   if (qi >= rows_do) return;
   const float r = sum == 0.f ? 0.f : 1.f / sum;
-  uint16_t *dst = p.out + (size_t)(first + qi) * p.ldo + (head * p.group + flat % p.group) * D + d;
+  uint16_t *dst = p.out + (size_t)(first + qi) * p.ldo + (head * p.group + flat - qi * p.group) * D + d;
   *reinterpret_cast<uint2 *>(dst) =
       make_uint2(f32_to_bf16_rne(acc.x * r) | ((uint32_t)f32_to_bf16_rne(acc.y * r) << 16),
                  f32_to_bf16_rne(acc.z * r) | ((uint32_t)f32_to_bf16_rne(acc.w * r) << 16));

@@ -118,29 +118,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
 }
 __device__ __forceinline__ void dc_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kDcWarps) : "memory"); }
 
-// A wait that gives up after a second, or at once when another warp has: the
-// item loop then runs to its end without touching the stages.
-__device__ __forceinline__ bool dc_wait(uint32_t bar, uint32_t parity, volatile int *abort, int *err) {
-  if (*abort) return false;
-  if (mbar_wait_bounded_warp(bar, parity)) return true;
-  *abort = 1;
-  atomicCAS(err, 0, kErrWaitTimeout);
-  return false;
-}
-
-template <int N>
-__device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N]) {
-  if constexpr (N == 4) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(p);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-  } else if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-    w[0] = v.x, w[1] = v.y;
-  } else {
-    w[0] = *reinterpret_cast<const uint32_t *>(p);
-  }
-}
-
 template <int NJ, int NB>
 struct DcLayout {
   static constexpr int D = 32 * NJ, cols = 8 * NB;
@@ -282,7 +259,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
           at = (lane >> 1) * half + (lane & 1) * c;
           if (mine) src += (lane >> 1 ? a.g.vc_off : 0) + (lane & 1 ? a.g.kp_off : 0) + second * bytes;
         }
-        ok = dc_wait(bar_empty + 8 * slot, phase ^ 1, abort, a.err);
+        ok = attn_wait(bar_empty + 8 * slot, phase ^ 1, abort, a.err);
         if (!ok) break;
         const uint32_t total = __reduce_add_sync(0xffffffffu, mine ? bytes : 0u);
         if (lane == 0) mbar_arrive_expect_tx(bar_full + 8 * slot, total);
@@ -324,12 +301,12 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
     int pos[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int flat = it.cb * NC + 8 * nb + g, qi = flat / a.group;
+      const int flat = it.cb * NC + 8 * nb + g, qi = attn_row(a, flat);
       uint4 w[NJ];
 #pragma unroll
       for (int j = 0; j < NJ; ++j) w[j] = make_uint4(0, 0, 0, 0);
       if (qi < s.rows_do) {
-        const uint16_t *src = a.q + (size_t)(s.first + qi) * a.ldq + (it.head * a.group + flat % a.group) * D + 8 * q4;
+        const uint16_t *src = a.q + (size_t)(s.first + qi) * a.ldq + (it.head * a.group + flat - qi * a.group) * D + 8 * q4;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) w[j] = __ldcg(reinterpret_cast<const uint4 *>(src + 32 * j));
       }
@@ -365,7 +342,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
 #pragma unroll
         for (int j = 0; j < NJ; ++j) qs[nb][j][c] = __shfl_sync(0xffffffffu, gs[j], from);
         cs[nb][c] = pow2f(-__shfl_sync(0xffffffffu, sh, from)) * 0x1p24f * a.scale_log2;
-        const int ci = col / a.group;
+        const int ci = attn_row(a, col);
         pos[nb][c] = ci < s.rows_do ? s.len - s.rows + ci : -1;
       }
     }
@@ -383,7 +360,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
 
     for (int t0 = t_start; t0 < t_end; t0 += kDcStage) {
       if (!dc_stage_visible(s, t0)) continue;
-      const bool ready = dc_wait(bar_full + 8 * slot, phase, abort, a.err);
+      const bool ready = attn_wait(bar_full + 8 * slot, phase, abort, a.err);
       const int tw = t0 + 16 * warp;                     // this warp's 16 tokens
       if (ready && tw < s.len && (tw + 16 > s.lo || tw < s.sinks)) {
         const uint8_t *st = sm + slot * L::stage;

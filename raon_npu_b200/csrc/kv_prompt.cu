@@ -6,11 +6,16 @@
 //   S_t = Q_t K^T            f16 x f16 -> f32 in tensor memory
 //   P_t = 2^(c S_t - ref)    one thread a row; f16, written over S_t
 //   O_t = O_t + P_t V        P from tensor memory, f32 accumulators there
-// Roles: two warpgroups of softmax threads (a tile each; their threads also
-// bring the query rows in and write the results), one warpgroup that
-// dequantises K and V into two shared-memory stages, one warp that issues the
-// products.  The issuing thread takes whatever is ready of the two tiles, so
-// one tile's products run while the other tile's softmax does.
+// Roles: eight softmax warps (a tile for four of them, one thread a row; they
+// also write the results), four warps that make Q, K and V f16 in shared memory,
+// one that copies the packed K and V in, one that issues the products, one that
+// finds the items.  A tile's next scores follow its values of this block, so a
+// tile's softmax has the time of the other's products.  CTAs are persistent and
+// every role goes straight from one item to the next, so the next item's query
+// rows and blocks come in while the last one's results go out.
+// The roles' loops are rolled and short on purpose: with the scores of a row in
+// registers and everything unrolled, the roles together outgrew the instruction
+// cache and each of them, the issuing warp first, ran at the speed of its misses.
 //
 // Numbers: K, V, Q and P are f16 (11 bits; one rounding each).  Q is scaled by
 // a power of two per row, K per block and V by a power of two that follows the
@@ -29,54 +34,86 @@
 namespace rc {
 
 constexpr int kPrRows = 128;                         // rows of a tile, tokens of a block
-constexpr int kPrThreads = 13 * 32;
+constexpr int kPrThreads = 512;
 constexpr int kPrInfo = 4;                           // blocks whose exponents are kept
+constexpr int kPrRaw = 3;                            // packed K or V blocks on their way in
 constexpr uint32_t kPrTmemCols = 512;
+// The rows of an item and the blocks of tokens they see.
+struct PrItem {
+  int b, head, flat0;                     // sequence (-1: no more items), kv head, first of the item's 256 rows
+  int first, rows, rows_do, len;
+  int lo, sinks, sink_blocks, blk_lo, blocks;
+  int tiles;
+};
 
 template <int NJ>
 struct PrLayout {
-  static constexpr int D = 32 * NJ, halves = D / 64;              // 128-byte column blocks of a row
+  static constexpr int D = 32 * NJ;
   static constexpr int tile = kPrRows * D * 2;
   static constexpr int o_q = 0, o_k = 2 * tile, o_v = o_k + 2 * tile;
-  static constexpr int o_poison = o_v + 2 * tile;                 // [kPrInfo][128] group masks of NaN values
+  static constexpr int o_poison = o_v + 2 * tile;                 // [kPrInfo][128] group masks of NaN values, bit 7: NaN key
   static constexpr int o_info = o_poison + kPrInfo * kPrRows;     // [kPrInfo]{K exponent, V exponent, poisoned, -}
   static constexpr int o_red = o_info + kPrInfo * 16;             // [2][4 warps]{K, V}
-  static constexpr int o_bar = o_red + 64;
-  static constexpr int n_bars = 16;
+  static constexpr int o_crow = o_red + 64;                       // [2 items][256] score scales, NaN for a row that is
+  static constexpr int o_item = o_crow + 2 * 2 * kPrRows * 4;     // [2] items
+  static constexpr int o_bar = o_item + 2 * 64;
+  static constexpr int n_bars = 32;
   static constexpr int o_misc = o_bar + 8 * n_bars;               // tensor memory address, abort word
-  static constexpr int bytes = o_misc + 16 + 1024;                // and the alignment
+  static constexpr int o_prefix = o_misc + 16;                    // [n_seqs / 32 + 1] items of the sequences before
+  static constexpr int o_raw = (o_prefix + (kKvMaxSeqs / 32 + 1) * 4 + 127) / 128 * 128;
+  static constexpr int raw = kPrRows * D * 5 / 8;                 // packed K or V of a block
+  static constexpr int bytes = o_raw + kPrRaw * raw + 1024;       // and the alignment
   static constexpr uint32_t s_col = 0, o_col = 2 * kPrRows;       // tensor memory: S0 S1 O0 O1
 };
+static_assert(sizeof(PrItem) <= 64, "an item's slot");
+static_assert(PrLayout<4>::bytes <= kGemvSmemLimit, "shared memory of an SM");
 
 __device__ __forceinline__ void pr_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pr_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ bool pr_elect() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
 __device__ __forceinline__ void pr_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void pr_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for the loads; ``v`` (the last one's values) is touched so that nothing uses it earlier.
+__device__ __forceinline__ void pr_wait_ld(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]),
+                 "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
+                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]),
+                 "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                 "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
+                 "+r"(v[30]), "+r"(v[31])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void pr_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Operand tiles in the 128-byte swizzle: rows 128 B apart, 8-row groups 1024 B
-// apart; 64-value column blocks one tile half apart.
-__device__ __forceinline__ uint64_t pr_desc(uint32_t saddr, uint32_t lead) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Descriptor of an operand tile in the 128-byte swizzle: rows 128 B apart, 8-row groups 1024 B apart, 64-value column
+// blocks ``lead`` bytes apart (for an N-major tile).  The low word; the high one is the same for all.
+__device__ __forceinline__ uint32_t pr_desc(uint32_t saddr, uint32_t lead) {
+  return ((saddr >> 4) & 0x3FFF) | ((lead >> 4) << 16);
 }
+constexpr uint32_t kPrDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
 // f32 accumulator, f16 operands, M = 128; B K-major (QK^T) or N-major (PV).
 __device__ constexpr uint32_t pr_idesc(int n, bool b_n_major) {
   return (1u << 4) | ((b_n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kPrRows >> 4) << 24);
 }
-__device__ __forceinline__ void pr_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void pr_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kPrDescHigh));
 }
-__device__ __forceinline__ void pr_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void pr_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc));
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kPrDescHigh));
 }
 __device__ __forceinline__ void pr_ld32(uint32_t addr, uint32_t (&v)[32]) {
   asm volatile(
@@ -106,62 +143,63 @@ __device__ __forceinline__ void pr_st16(uint32_t addr, const uint32_t (&v)[16]) 
       : "memory");
 }
 
-// The rows of an item and the blocks of tokens they see.
-struct PrItem {
-  int b, head, flat0;                     // sequence, kv head, first row of the item's 256
-  int first, rows, rows_do, len;
-  int lo, sinks, sink_blocks, blk_lo, blocks;
-};
 __device__ __forceinline__ int pr_block(const PrItem &it, int j) {   // first token of the j-th block
   return (j < it.sink_blocks ? j : it.blk_lo + j - it.sink_blocks) * kPrRows;
 }
-
-// Item blockIdx.x: sequences in order, a sequence's last rows (the longest
-// items) first, kv heads innermost.  Computed by warp 0, shared by all.
-__device__ __forceinline__ bool pr_item(const AttnParams &p, int lane, PrItem &it) {
-  const int rows_item = 2 * kPrRows;
-  int i = blockIdx.x;
-  for (int b0 = 0; b0 < p.b.n_seqs; b0 += 32) {
-    int first = 0, rows = 0, rows_do = 0, len = 0, n = 0;
-    if (b0 + lane < p.b.n_seqs) {
-      attn_seq(p, b0 + lane, first, rows, rows_do, len);
-      n = (int)(((long long)rows_do * p.group + rows_item - 1) / rows_item) * p.g.heads;
-    }
-    int run = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += u;
-    }
-    const unsigned in = __ballot_sync(0xffffffffu, i < run);
-    if (in) {
-      const int src = __ffs(in) - 1;
-      const int start = __shfl_sync(0xffffffffu, run - n, src), count = __shfl_sync(0xffffffffu, n, src);
-      it.b = b0 + src;
-      it.first = __shfl_sync(0xffffffffu, first, src);
-      it.rows = __shfl_sync(0xffffffffu, rows, src);
-      it.rows_do = __shfl_sync(0xffffffffu, rows_do, src);
-      it.len = __shfl_sync(0xffffffffu, len, src);
-      const int r = i - start;
-      it.head = r % p.g.heads;
-      it.flat0 = (count / p.g.heads - 1 - r / p.g.heads) * rows_item;
-      const int base = it.len - it.rows;                                   // position of row 0
-      const int p_first = base + it.flat0 / p.group;
-      const int p_last = base + min(it.rows_do - 1, (it.flat0 + rows_item - 1) / p.group);
-      it.lo = p.window > 0 ? max(0, p_first - p.window + 1) : 0;
-      it.sinks = p.window > 0 ? min(p.sinks, it.lo) : 0;
-      it.blk_lo = it.lo / kPrRows;
-      it.sink_blocks = min((it.sinks + kPrRows - 1) / kPrRows, it.blk_lo);
-      const int end = p_last < 0 ? 0 : (p_last + kPrRows) / kPrRows;       // blocks up to the last visible token
-      it.blocks = p_last < 0 ? 0 : it.sink_blocks + max(0, end - it.blk_lo);
-      return true;
-    }
-    i -= __shfl_sync(0xffffffffu, run, 31);
-  }
-  return false;
+__device__ __forceinline__ int pr_items(const AttnParams &p, int rows_do) {
+  return (rows_do * p.group + 2 * kPrRows - 1) / (2 * kPrRows) * p.g.heads;
 }
 
-// Exponents of 128 tokens' params: the larger of the scales' and of minima more than 2^19 times as large.
+// Item i: sequences in order, a sequence's last rows (the longest items) first, kv heads innermost.  By a warp:
+// ``prefix`` has the items before every 32nd sequence.
+__device__ __forceinline__ PrItem pr_item(const AttnParams &p, const int *prefix, int i, int lane) {
+  int lo = 0, hi = (p.b.n_seqs - 1) / 32;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] <= i) lo = mid;
+    else hi = mid - 1;
+  }
+  PrItem it;
+  it.first = it.rows = it.rows_do = it.len = 0;
+  if (32 * lo + lane < p.b.n_seqs) attn_seq(p, 32 * lo + lane, it.first, it.rows, it.rows_do, it.len);
+  const int mine = pr_items(p, it.rows_do);
+  int run = mine;
+#pragma unroll 1
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += u;
+  }
+  i -= prefix[lo];
+  const int src = __ffs(__ballot_sync(0xffffffffu, i < run)) - 1;      // there is one: i < all items
+  it.b = 32 * lo + src;
+  it.first = __shfl_sync(0xffffffffu, it.first, src);
+  it.rows = __shfl_sync(0xffffffffu, it.rows, src);
+  it.rows_do = __shfl_sync(0xffffffffu, it.rows_do, src);
+  it.len = __shfl_sync(0xffffffffu, it.len, src);
+  const int count = __shfl_sync(0xffffffffu, mine, src), r = i - __shfl_sync(0xffffffffu, run - mine, src);
+  it.head = r % p.g.heads;
+  it.flat0 = (count / p.g.heads - 1 - r / p.g.heads) * 2 * kPrRows;
+  it.tiles = it.rows_do * p.group - it.flat0 > kPrRows ? 2 : 1;
+  const int base = it.len - it.rows;                                   // position of row 0
+  const int p_first = base + attn_row(p, it.flat0);
+  const int p_last = base + min(it.rows_do - 1, attn_row(p, it.flat0 + 2 * kPrRows - 1));
+  it.lo = p.window > 0 ? max(0, p_first - p.window + 1) : 0;
+  it.sinks = p.window > 0 ? min(p.sinks, it.lo) : 0;
+  it.blk_lo = it.lo / kPrRows;
+  it.sink_blocks = min((it.sinks + kPrRows - 1) / kPrRows, it.blk_lo);
+  const int end = p_last < 0 ? 0 : p_last / kPrRows + 1;               // blocks up to the last visible token
+  it.blocks = p_last < 0 ? 0 : it.sink_blocks + max(0, end - it.blk_lo);
+  return it;
+}
+// Token t is visible to a row of the item.
+__device__ __forceinline__ bool pr_seen_by_item(const PrItem &it, int t) { return t < it.len && (t >= it.lo || t < it.sinks); }
+
+// The k-th item of this CTA: rounds over the grid, every second one backwards, which evens out falling costs.
+__device__ __forceinline__ int pr_turn(int k) {
+  return k * (int)gridDim.x + (k & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+}
+
+// Exponents of a token's params: the larger of the scales' and of minima more than 2^19 times as large.
 template <int NJ>
 __device__ __forceinline__ int pr_exponent(const uint32_t (&par)[NJ]) {
   int e = 0;
@@ -173,20 +211,6 @@ __device__ __forceinline__ int pr_exponent(const uint32_t (&par)[NJ]) {
   return e;
 }
 __device__ __forceinline__ int pr_shift(int e) { return max(-126, min(122 - e, 106)); }
-
-template <int N>
-__device__ __forceinline__ void ldg_words(const uint8_t *p, uint32_t (&w)[N]) {
-  if constexpr (N % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(p + 4 * i));
-      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
-    }
-  } else {
-    const uint2 v = __ldcg(reinterpret_cast<const uint2 *>(p));
-    w[0] = v.x, w[1] = v.y;
-  }
-}
 
 // Eight codes of a word into four f16x2 {nibble i, nibble i + 4}, scaled.
 __device__ __forceinline__ uint4 pr_unpack(uint32_t w, uint32_t s2, uint32_t m2) {
@@ -200,25 +224,100 @@ __device__ __forceinline__ uint32_t pr_chunk(int r, int c) {
 }
 
 struct PrBars {
-  uint32_t q, kfull, kempty, vfull, vempty, sfull, pfull, odone, drain;
+  uint32_t item_full, item_empty, q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_empty, drain, vote, raw_full, raw_empty;
 };
 
-__device__ __forceinline__ bool pr_wait(uint32_t bar, uint32_t parity, volatile int *abort, int *err) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = global_timer_ns();
-  while (!*abort) {
+// Of columns 32 k .. 32 k + 31, those a row sees: column <= c_hi, and > c_lo or < c_sink.
+__device__ __forceinline__ uint32_t pr_seen(int k, int c_hi, int c_lo, int c_sink) {
+  const int hi = c_hi - 32 * k, lo = max(c_lo, -64) - 32 * k, sk = c_sink - 32 * k;
+  const uint32_t upto = hi < 0 ? 0u : hi >= 31 ? ~0u : (2u << hi) - 1u;
+  const uint32_t past = lo < 0 ? ~0u : lo >= 31 ? 0u : ~((2u << lo) - 1u);
+  const uint32_t first = sk <= 0 ? 0u : sk >= 32 ? ~0u : (1u << sk) - 1u;
+  return upto & (past | first);
+}
+
+__device__ __forceinline__ void pr_scale8(uint32_t addr, float by) {
+  uint32_t v[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])
+               :
+               : "memory");
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * by);
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+__device__ __forceinline__ uint64_t pr_pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void pr_split(uint64_t v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t pr_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t pr_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Largest score of this thread's row (in the product's units).
+template <bool MASKED>
+__device__ __forceinline__ float pr_top(uint32_t s_at, int c_hi, int c_lo, int c_sink) {
+  float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-    for (int i = 0; i < 32; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
-    if (global_timer_ns() - t0 > 1000000000ull) {
-      *abort = 1;
-      atomicCAS(err, 0, kErrWaitTimeout);
+  for (int k = 0; k < 4; ++k) {
+    uint32_t v[32];
+    pr_ld32(s_at + 32 * k, v);
+    const uint32_t seen = MASKED ? pr_seen(k, c_hi, c_lo, c_sink) : ~0u;
+    pr_wait_ld(v);
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const float x0 = MASKED && !(seen >> e & 1) ? -INFINITY : __uint_as_float(v[e]);
+      const float x1 = MASKED && !(seen >> (e + 1) & 1) ? -INFINITY : __uint_as_float(v[e + 1]);
+      a[(e >> 1) & 3] = fmaxf(fmaxf(a[(e >> 1) & 3], x0), x1);
     }
   }
-  return false;
+  return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
-__device__ __forceinline__ bool pr_wait_warp(uint32_t bar, uint32_t parity, volatile int *abort, int *err) {
-  return __all_sync(0xffffffffu, pr_wait(bar, parity, abort, err));
+
+// Weights 2^(c S + minus) of this thread's row, f16, over the scores; returns their sum.
+template <bool MASKED>
+__device__ __forceinline__ float pr_weights(uint32_t s_at, float c, float minus, int c_hi, int c_lo, int c_sink) {
+  const uint64_t c2 = pr_pair(c, c), m2 = pr_pair(minus, minus);
+  uint64_t sum[2] = {0, 0};
+#pragma unroll 1
+  for (int k = 0; k < 4; ++k) {
+    uint32_t v[32], w[16];
+    pr_ld32(s_at + 32 * k, v);
+    const uint32_t seen = MASKED ? pr_seen(k, c_hi, c_lo, c_sink) : ~0u;
+    pr_wait_ld(v);
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      float x0, x1;
+      pr_split(pr_fma2(pr_pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), c2, m2), x0, x1);
+      if (MASKED && !(seen >> e & 1)) x0 = -INFINITY;
+      if (MASKED && !(seen >> (e + 1) & 1)) x1 = -INFINITY;
+      x0 = ex2(x0);
+      x1 = ex2(x1);
+      sum[(e >> 1) & 1] = pr_add2(sum[(e >> 1) & 1], pr_pair(x0, x1));
+      w[e / 2] = pack_f16x2(x0, x1);
+    }
+    pr_st16(s_at + 16 * k, w);
+  }
+  float a, b;
+  pr_split(pr_add2(sum[0], sum[1]), a, b);
+  return a + b;
 }
 
 template <int NJ>
@@ -226,45 +325,57 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
   using L = PrLayout<NJ>;
   constexpr int D = L::D;
   extern __shared__ uint8_t pr_raw[];
-  __shared__ PrItem s_item;
-  __shared__ int s_have;
   uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pr_raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t bar0 = smem_addr(sm + L::o_bar);
-  const PrBars bars{bar0, bar0 + 8, bar0 + 24, bar0 + 40, bar0 + 56, bar0 + 72, bar0 + 88, bar0 + 104, bar0 + 120};
+  const PrBars bars{bar0,       bar0 + 16,  bar0 + 32,  bar0 + 48,  bar0 + 64,  bar0 + 80, bar0 + 96,
+                    bar0 + 112, bar0 + 128, bar0 + 144, bar0 + 160, bar0 + 176, bar0 + 192, bar0 + 200, bar0 + 208, bar0 + 232};
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + L::o_misc);
   volatile int *abort = reinterpret_cast<volatile int *>(sm + L::o_misc + 4);
   int4 *info = reinterpret_cast<int4 *>(sm + L::o_info);
   uint8_t *poison = sm + L::o_poison;
+  float *crow = reinterpret_cast<float *>(sm + L::o_crow);
+  int *prefix = reinterpret_cast<int *>(sm + L::o_prefix);
+  if (tid == 0) {
+    *abort = 0;
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bars.item_full + 8 * s, 1);
+      mbar_init(bars.item_empty + 8 * s, 14);            // eight softmax warps, four that make operands, copies, products
+      mbar_init(bars.q_full + 8 * s, kPrRows);
+      mbar_init(bars.q_empty + 8 * s, 1);
+      mbar_init(bars.k_full + 8 * s, kPrRows);
+      mbar_init(bars.k_empty + 8 * s, 1);
+      mbar_init(bars.v_full + 8 * s, kPrRows);
+      mbar_init(bars.v_empty + 8 * s, 1);
+      mbar_init(bars.s_full + 8 * s, 1);
+      mbar_init(bars.p_full + 8 * s, 4);
+      mbar_init(bars.o_done + 8 * s, 1);
+      mbar_init(bars.o_empty + 8 * s, 4);
+    }
+    mbar_init(bars.drain, 1);
+    mbar_init(bars.vote, 4);
+    for (int s = 0; s < kPrRaw; ++s) {
+      mbar_init(bars.raw_full + 8 * s, 1);
+      mbar_init(bars.raw_empty + 8 * s, 4);
+    }
+    mbar_fence_init();
+  }
   pdl_launch_dependents();
   pdl_wait_prior();
-  if (warp == 0) {
-    PrItem it;
-    const bool have = pr_item(p, lane, it);
-    if (lane == 0) {
-      s_have = have;
-      if (have) s_item = it;
-      *abort = 0;
-      const int tiles = have && (it.rows_do * p.group - it.flat0) > kPrRows ? 2 : 1;
-      mbar_init(bars.q, kPrRows * 2);
-      for (int s = 0; s < 2; ++s) {
-        mbar_init(bars.kfull + 8 * s, kPrRows);
-        mbar_init(bars.kempty + 8 * s, tiles);
-        mbar_init(bars.vfull + 8 * s, kPrRows);
-        mbar_init(bars.vempty + 8 * s, tiles);
-        mbar_init(bars.sfull + 8 * s, 1);
-        mbar_init(bars.pfull + 8 * s, kPrRows);
-        mbar_init(bars.odone + 8 * s, 1);
-      }
-      mbar_init(bars.drain, 1);
-      mbar_fence_init();
-    }
+  // items of every 32 sequences, then of all before them
+#pragma unroll 1
+  for (int b0 = 32 * warp; b0 < p.b.n_seqs; b0 += kPrThreads) {
+    int first, rows, rows_do = 0, len;
+    if (b0 + lane < p.b.n_seqs) attn_seq(p, b0 + lane, first, rows, rows_do, len);
+    const int all = (int)__reduce_add_sync(0xffffffffu, (uint32_t)pr_items(p, rows_do));
+    if (lane == 0) prefix[b0 / 32 + 1] = all;
   }
   __syncthreads();
-  if (!s_have) return;
-  const PrItem it = s_item;
-  const int tiles = it.rows_do * p.group - it.flat0 > kPrRows ? 2 : 1;
-  if (warp == 12 && it.blocks) {
+  if (tid == 0) {
+    prefix[0] = 0;
+#pragma unroll 1
+    for (int g = 0; g < (p.b.n_seqs + 31) / 32; ++g) prefix[g + 1] += prefix[g];
+  } else if (warp == 12) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
                  "r"(kPrTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -272,164 +383,107 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
   pr_fence_before();
   __syncthreads();
   pr_fence_after();
-  const uint32_t tmem = it.blocks ? *tmem_slot : 0;
+  const uint32_t tmem = *tmem_slot;
+  auto item_done = [&](int k) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bars.item_empty + 8 * (k & 1));
+  };
 
   if (warp < 8) {
-    // ------------------------------------------------- query rows, softmax --
+    // ------------------------------------------------------------- softmax --
     const int t = warp >> 2, row = tid & (kPrRows - 1);
-    const int flat = it.flat0 + t * kPrRows + row, qi = flat / p.group;
-    const bool live = qi < it.rows_do;
-    const int pos = it.len - it.rows + qi;
-    const size_t head_at = (size_t)(it.head * p.group + flat % p.group) * D;
-    float l = 0.f;
-    int fv = 0;
-    uint32_t nan_groups = 0;
-    if (it.blocks) {
-      float c_row;
-      {
-        uint4 w[4 * NJ];
-#pragma unroll
-        for (int i = 0; i < 4 * NJ; ++i) w[i] = make_uint4(0, 0, 0, 0);
-        if (live) {
-          const uint4 *src = reinterpret_cast<const uint4 *>(p.q + (size_t)(it.first + qi) * p.ldq + head_at);
-#pragma unroll
-          for (int i = 0; i < 4 * NJ; ++i) w[i] = __ldcg(src + i);
-        }
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 4 * NJ; ++i) {
-          const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7FFFu, (u[e] >> 16) & 0x7FFFu));
-        }
-        const int sh = top < (15u << 7) ? 126 : 141 - (int)(top >> 7);
-        const float mul = p.scale_log2 < 0.f ? -pow2f(sh) : pow2f(sh);   // the sign of the scale goes into Q
-        c_row = pow2f(-sh) * fabsf(p.scale_log2);
-#pragma unroll
-        for (int i = 0; i < 4 * NJ; ++i) {
-          // dims 8i .. 8i+7 = 32j + 8q ..: chunk q * NJ + j
-          const int j = i / 4, q = i % 4;
-          const float x[8] = {bf16_lo_f32(w[i].x) * mul, bf16_hi_f32(w[i].x) * mul, bf16_lo_f32(w[i].y) * mul,
-                              bf16_hi_f32(w[i].y) * mul, bf16_lo_f32(w[i].z) * mul, bf16_hi_f32(w[i].z) * mul,
-                              bf16_lo_f32(w[i].w) * mul, bf16_hi_f32(w[i].w) * mul};
-          *reinterpret_cast<uint4 *>(sm + L::o_q + t * L::tile + pr_chunk(row, q * NJ + j)) =
-              make_uint4(pack_f16x2(x[0], x[4]), pack_f16x2(x[1], x[5]), pack_f16x2(x[2], x[6]), pack_f16x2(x[3], x[7]));
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(bars.q);
-      if (t < tiles) {
-        const uint32_t lane_at = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t s_at = tmem + lane_at + L::s_col + t * kPrRows, o_at = tmem + lane_at + L::o_col + t * D;
-        // positions of the tile's rows, for the blocks that need no mask
-        const int base = it.len - it.rows, last_flat = it.rows_do * p.group - 1;
-        const int p_min = base + min(it.flat0 + t * kPrRows, last_flat) / p.group;
-        const int p_max = base + min(it.flat0 + t * kPrRows + kPrRows - 1, last_flat) / p.group;
-        float ref = -INFINITY;
+    const uint32_t lane_at = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    const uint32_t s_at = lane_at + L::s_col + t * kPrRows, o_at = lane_at + L::o_col + t * D;
+    const uint32_t bar_s = bars.s_full + 8 * t, bar_p = bars.p_full + 8 * t, bar_o = bars.o_done + 8 * t;
+    int n = 0, done = 0;                                  // blocks of all items so far; this tile's
+#pragma unroll 1
+    for (int k = 0;; ++k) {
+      if (!attn_wait(bars.item_full + 8 * (k & 1), (k >> 1) & 1, abort, p.err)) break;
+      const PrItem *it = reinterpret_cast<const PrItem *>(sm + L::o_item + 64 * (k & 1));
+      if (it->b < 0) break;
+      const int blocks = it->blocks;
+      if (t < it->tiles) {
+        const int flat0 = it->flat0 + t * kPrRows, base = it->len - it->rows;
+        // positions: of this row, and of the tile's rows, for the blocks that need no mask
+        const int last_flat = it->rows_do * p.group - 1;
+        const int pos = base + attn_row(p, flat0 + row);
+        const int p_min = base + attn_row(p, min(flat0, last_flat));
+        const int p_max = base + attn_row(p, min(flat0 + kPrRows - 1, last_flat));
+        float c_row = 0.f, ref = -INFINITY, l = 0.f;
+        int fv = 0;
+        uint32_t nan_groups = 0;
         bool ok = true;
-        for (int j = 0; j < it.blocks && ok; ++j) {
-          const int t0 = pr_block(it, j);
+#pragma unroll 1
+        for (int j = 0; j < blocks; ++j, ++done) {
+          const int t0 = pr_block(*it, j);
           const bool masked = !(t0 + kPrRows - 1 <= p_min &&
                                 (p.window <= 0 || t0 > p_max - p.window || t0 + kPrRows <= p.sinks));
-          const int c_hi = pos - t0, c_lo = p.window > 0 ? c_hi - p.window : INT_MIN, c_sink = p.sinks - t0;
-          ok = pr_wait_warp(bars.sfull + 8 * t, j & 1, abort, p.err);
+          ok = attn_wait(bar_s, done & 1, abort, p.err);
           if (!ok) break;
           pr_fence_after();
-          const int4 f = info[j % kPrInfo];
-          const float c = c_row * pow2f(-f.x);
-          float top = -INFINITY;
-          uint32_t v[32];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            pr_ld32(s_at + 32 * k, v);
-            pr_wait_ld();
-            float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (masked) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const int col = 32 * k + e;
-                const bool see = col <= c_hi && (col > c_lo || col < c_sink);
-                a[e & 3] = fmaxf(a[e & 3], see ? __uint_as_float(v[e]) : -INFINITY);
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) a[e & 3] = fmaxf(a[e & 3], __uint_as_float(v[e]));
-            }
-            top = fmaxf(top, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
+          if (j == 0) {
+            c_row = crow[(k & 1) * 2 * kPrRows + t * kPrRows + row];
+            if (c_row != c_row) c_row = 0.f, nan_groups = (1u << NJ) - 1u;
           }
+          const int4 f = info[(n + j) % kPrInfo];
+          const float c = c_row * pow2f(-f.x);
+          const int c_hi = pos - t0, c_lo = p.window > 0 ? c_hi - p.window : INT_MIN, c_sink = p.sinks - t0;
+          const float top = masked ? pr_top<true>(s_at, c_hi, c_lo, c_sink) : pr_top<false>(s_at, 0, 0, 0);
           const float x_top = top == -INFINITY ? -INFINITY : top * c;
-          const bool move = x_top > ref + kAttnSlack;
-          if (__any_sync(0xffffffffu, move || (j > 0 && f.y != fv))) {
+          if (__any_sync(0xffffffffu, x_top > ref + kAttnSlack || f.y != fv)) {
             float by = 1.f;
-            if (move) {
+            if (x_top > ref + kAttnSlack) {
               by = exp2f(ref - x_top);
               ref = x_top;
             }
             l *= by;
             if (j > 0) {
               by *= pow2f(max(f.y - fv, -126));
-              ok = pr_wait_warp(bars.odone + 8 * t, (j - 1) & 1, abort, p.err);
+              ok = attn_wait(bar_o, (done - 1) & 1, abort, p.err);
               if (!ok) break;
               pr_fence_after();
 #pragma unroll 1
-              for (int k = 0; k < D / 32; ++k) {
-                pr_ld32(o_at + 32 * k, v);
-                pr_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * by);
-                pr_st32(o_at + 32 * k, v);
-              }
-              pr_wait_st();
+              for (int i = 0; i < D / 8; ++i) pr_scale8(o_at + 8 * i, by);
             }
+            fv = f.y;
           }
-          fv = f.y;
           const float minus = ref == -INFINITY ? 0.f : kAttnLift - ref;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            pr_ld32(s_at + 32 * k, v);
-            pr_wait_ld();
-            uint32_t w[16];
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              float x0 = fmaf(__uint_as_float(v[e]), c, minus), x1 = fmaf(__uint_as_float(v[e + 1]), c, minus);
-              if (masked) {
-                const int col = 32 * k + e;
-                if (!(col <= c_hi && (col > c_lo || col < c_sink))) x0 = -INFINITY;
-                if (!(col + 1 <= c_hi && (col + 1 > c_lo || col + 1 < c_sink))) x1 = -INFINITY;
-              }
-              x0 = ex2(x0);
-              x1 = ex2(x1);
-              sum[(e >> 1) & 3] += x0 + x1;
-              w[e / 2] = pack_f16x2(x0, x1);
-            }
-            pr_st16(s_at + 16 * k, w);
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          l += masked ? pr_weights<true>(s_at, c, minus, c_hi, c_lo, c_sink) : pr_weights<false>(s_at, c, minus, 0, 0, 0);
           if (f.z) {
             // groups of this block that hold NaN, in tokens that this row sees
+#pragma unroll 1
             for (int col = 0; col < kPrRows; ++col) {
               const bool see = col <= c_hi && (col > c_lo || col < c_sink);
-              if (see) nan_groups |= poison[(j % kPrInfo) * kPrRows + col];
+              const uint32_t m = poison[((n + j) % kPrInfo) * kPrRows + col];
+              if (see) nan_groups |= m & 0x80 ? (1u << NJ) - 1u : m;
             }
           }
           pr_wait_st();
           pr_fence_before();
-          mbar_arrive(bars.pfull + 8 * t);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_p);
         }
-        if (ok) ok = pr_wait_warp(bars.odone + 8 * t, (it.blocks - 1) & 1, abort, p.err);
-        pr_fence_after();
+        // results; zeros where there are no blocks
+        if (blocks && ok) ok = attn_wait(bar_o, (done - 1) & 1, abort, p.err);
         if (ok) {
-          // columns 8W + 2i + o hold dim 32 (j + o) + 4 g + i, W = (g NJ + j) / 2; 32 columns cover 16 / NJ g's
+          pr_fence_after();
+          const int flat = flat0 + row, qi = attn_row(p, flat);
+          const bool live = qi < it->rows_do;
+          uint16_t *dst = p.out + (size_t)(it->first + qi) * p.ldo + (size_t)(it->head * p.group + flat - qi * p.group) * D;
+          // columns 8W + 2i + o hold dim 32 (j + o) + 4 g + i, W = (g NJ + j) / 2; 32 columns cover 8 / NJ g's
+          constexpr int kPer = 8 / NJ;
           const float r = l == 0.f ? 0.f : 1.f / l, un = pow2f(-fv);
-          uint16_t *dst = p.out + (size_t)(it.first + qi) * p.ldo + head_at;
 #pragma unroll 1
-          for (int k = 0; k < D / 32; ++k) {
+          for (int i = 0; i < D / 32; ++i) {
             uint32_t v[32];
-            pr_ld32(o_at + 32 * k, v);
-            pr_wait_ld();
+            if (blocks) {
+              pr_ld32(o_at + 32 * i, v);
+              pr_wait_ld(v);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = 0;
+            }
             if (live) {
-              constexpr int kPer = 8 / NJ;               // g's of 32 columns
 #pragma unroll
               for (int j = 0; j < NJ; ++j) {
                 const float bad = (nan_groups >> j) & 1 ? NAN : 0.f;
@@ -439,160 +493,324 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
                   const int c0 = 8 * ((g * NJ + j) / 2) + (j & 1);
                   float x[4];
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v[c0 + 2 * i]) * r * un + bad;
-                  w[2 * g] = f32_to_bf16_rne(x[0]) | ((uint32_t)f32_to_bf16_rne(x[1]) << 16);
-                  w[2 * g + 1] = f32_to_bf16_rne(x[2]) | ((uint32_t)f32_to_bf16_rne(x[3]) << 16);
+                  for (int e = 0; e < 4; ++e) x[e] = fmaf(__uint_as_float(v[c0 + 2 * e]) * r, un, bad);
+                  w[2 * g] = pack_bf16x2(x[0], x[1]);
+                  w[2 * g + 1] = pack_bf16x2(x[2], x[3]);
                 }
 #pragma unroll
                 for (int g = 0; g < 2 * kPer; g += 4)
-                  *reinterpret_cast<uint4 *>(dst + 32 * j + 4 * kPer * k + 2 * g) = make_uint4(w[g], w[g + 1], w[g + 2], w[g + 3]);
+                  *reinterpret_cast<uint4 *>(dst + 32 * j + 4 * kPer * i + 2 * g) = make_uint4(w[g], w[g + 1], w[g + 2], w[g + 3]);
               }
             }
           }
+          if (blocks) {
+            pr_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars.o_empty + 8 * t);
+          }
         }
       }
-    } else if (live && t < tiles) {
-      uint4 *dst = reinterpret_cast<uint4 *>(p.out + (size_t)(it.first + qi) * p.ldo + head_at);
-#pragma unroll
-      for (int i = 0; i < 4 * NJ; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+      n += blocks;
+      item_done(k);
     }
-  } else if (warp < 12 && it.blocks) {
-    // --------------------------------------------------------- dequantise --
+  } else if (warp < 12) {
+    // -------------------------------------------------- operands as f16 --
     const int row = tid & (kPrRows - 1), w4 = warp & 3;
-    uint32_t kc[4 * NJ], vc[4 * NJ], kp[NJ], vp[NJ];
     int2 *red = reinterpret_cast<int2 *>(sm + L::o_red);
-    auto fetch = [&](int j) {   // this thread's token of block j; zeros where nobody sees it
-      const int tok = pr_block(it, j) + row;
-      const uint8_t *blk = nullptr;
-      if (tok < it.len && (tok >= it.lo || tok < it.sinks)) blk = kv_head_block(p.g, p.b, it.b, tok, it.head, p.err);
-      if (blk) {
-        const int at = tok & (p.g.page - 1);
-        ldg_words<NJ>(blk + p.g.kp_off + at * NJ * 4, kp);
-        ldg_words<NJ>(blk + p.g.vp_off + at * NJ * 4, vp);
-        ldg_words<4 * NJ>(blk + at * (D / 2), kc);
-        ldg_words<4 * NJ>(blk + p.g.vc_off + at * (D / 2), vc);
-      } else {
-#pragma unroll
-        for (int i = 0; i < NJ; ++i) kp[i] = vp[i] = 0;
-#pragma unroll
-        for (int i = 0; i < 4 * NJ; ++i) kc[i] = vc[i] = 0;
-      }
-    };
+    // this row's codes and params within a packed block: the pages' parts one after the other
+    const uint32_t sub = (uint32_t)(row >> p.g.log2_page) * (p.g.head_bytes / 2);
+    const uint32_t o_codes = sub + (row & (p.g.page - 1)) * (D / 2);
+    const uint32_t o_par = sub + p.g.kp_off + (row & (p.g.page - 1)) * (NJ * 4);
+    int n = 0, uses0 = 0, uses1 = 0;                      // blocks so far; items of each tile so far
+    int slot = 0;                                         // of the packed blocks
+    uint32_t turn = 0;
     int v_exp = 0;
-    fetch(0);
-    // Every warp goes through every block's barrier, also after a wait has given up.
-    for (int j = 0; j < it.blocks; ++j) {
-      const int s = j & 1;
-      const uint32_t ph = (j >> 1) & 1;
-      // the block's exponents
-      uint32_t mask = 0;
+#pragma unroll 1
+    for (int k = 0;; item_done(k), ++k) {
+      if (!attn_wait(bars.item_full + 8 * (k & 1), (k >> 1) & 1, abort, p.err)) break;
+      const PrItem &it = *reinterpret_cast<const PrItem *>(sm + L::o_item + 64 * (k & 1));
+      if (it.b < 0) break;
+      if (it.blocks == 0) continue;
+      // the item's query rows, 4 NJ lanes a row
+#pragma unroll 1
+      for (int t = 0; t < it.tiles; ++t) {
+        const bool free = attn_wait(bars.q_empty + 8 * t, ((t ? uses1 : uses0) & 1) ^ 1, abort, p.err);
+        if (t) ++uses1;
+        else ++uses0;
+        if (!free) continue;
+        constexpr int kLanes = 4 * NJ, kAtOnce = 4;
+        const int i = row % kLanes;                       // dims 8i .. 8i+7 = 32j + 8q ..: chunk q * NJ + j
+#pragma unroll 1
+        for (int r0 = row / kLanes; r0 < kPrRows; r0 += kAtOnce * (kPrRows / kLanes)) {
+          uint4 w[kAtOnce];
 #pragma unroll
-      for (int i = 0; i < NJ; ++i)
-        if (((vp[i] >> 7) & 0xFF) == 0xFF || ((vp[i] >> 23) & 0xFF) == 0xFF) mask |= 1u << i, vp[i] = 0;
-      const int ke = (int)__reduce_max_sync(0xffffffffu, (uint32_t)pr_exponent<NJ>(kp));
-      const int ve = (int)__reduce_max_sync(0xffffffffu, (uint32_t)pr_exponent<NJ>(vp)) | (__any_sync(0xffffffffu, mask != 0) ? 0x1000 : 0);
-      if (lane == 0) red[s * 4 + w4] = make_int2(ke, ve);
-      asm volatile("bar.sync 2, %0;" ::"n"(kPrRows) : "memory");
-      int k_exp = 0, bad = 0;
+          for (int u = 0; u < kAtOnce; ++u) {
+            const int flat = it.flat0 + t * kPrRows + r0 + u * (kPrRows / kLanes), qi = attn_row(p, flat);
+            w[u] = make_uint4(0, 0, 0, 0);
+            if (r0 + u * (kPrRows / kLanes) < kPrRows && qi < it.rows_do)
+              w[u] = __ldcg(reinterpret_cast<const uint4 *>(p.q + (size_t)(it.first + qi) * p.ldq +
+                                                            (size_t)(it.head * p.group + flat - qi * p.group) * D) + i);
+          }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int2 e = red[s * 4 + i];
-        k_exp = max(k_exp, e.x);
-        v_exp = max(v_exp, e.y & 0xFFF);
-        bad |= e.y >> 12;
-      }
-      const int fk = pr_shift(k_exp), fvv = pr_shift(v_exp);
-      if (pr_wait_warp(bars.kempty + 8 * s, ph ^ 1, abort, p.err)) {
-        if (bad) poison[(j % kPrInfo) * kPrRows + row] = (uint8_t)mask;
-        if (row == 0) info[j % kPrInfo] = make_int4(fk, fvv, bad, 0);
-        const float up = pow2f(fk), up20 = up * 0x1p20f;
-        uint8_t *dst = sm + L::o_k + s * L::tile;
+          for (int u = 0; u < kAtOnce; ++u) {
+            const int r = r0 + u * (kPrRows / kLanes);
+            const uint32_t x4[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+            uint32_t top = 0;
 #pragma unroll
-        for (int g = 0; g < NJ; ++g) {
-          const uint32_t s2 = pack_f16x2(bf16_lo_f32(kp[g]) * up20, bf16_lo_f32(kp[g]) * up20);
-          const uint32_t m2 = pack_f16x2(bf16_hi_f32(kp[g]) * up, bf16_hi_f32(kp[g]) * up);
+            for (int e = 0; e < 4; ++e) top = max(top, max(x4[e] & 0x7FFFu, (x4[e] >> 16) & 0x7FFFu));
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint4 *>(dst + pr_chunk(row, q * NJ + g)) = pr_unpack(kc[q * NJ + g], s2, m2);
+            for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int sh = top < (15u << 7) ? 126 : 141 - (int)(top >> 7);   // largest value to [2^14, 2^15)
+            // the sign of the score scale goes into Q; a row that is not finite gives NaN, not its products
+            const float mul = top >= 0x7F80u ? 0.f : p.scale_log2 < 0.f ? -pow2f(sh) : pow2f(sh);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[2 * e] = top >= 0x7F80u ? 0.f : bf16_lo_f32(x4[e]) * mul;
+              x[2 * e + 1] = top >= 0x7F80u ? 0.f : bf16_hi_f32(x4[e]) * mul;
+            }
+            if (r < kPrRows) {
+              *reinterpret_cast<uint4 *>(sm + L::o_q + t * L::tile + pr_chunk(r, (i % 4) * NJ + i / 4)) =
+                  make_uint4(pack_f16x2(x[0], x[4]), pack_f16x2(x[1], x[5]), pack_f16x2(x[2], x[6]), pack_f16x2(x[3], x[7]));
+              if (i == 0)
+                crow[(k & 1) * 2 * kPrRows + t * kPrRows + r] = top >= 0x7F80u ? NAN : pow2f(-sh) * fabsf(p.scale_log2);
+            }
+          }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(bars.kfull + 8 * s);
+        mbar_arrive(bars.q_full + 8 * t);
       }
-      if (pr_wait_warp(bars.vempty + 8 * s, ph ^ 1, abort, p.err)) {
-        const float up = pow2f(fvv), up20 = up * 0x1p20f;
-        uint8_t *dst = sm + L::o_v + s * L::tile;
+
+#pragma unroll 1
+      for (int j = 0; j < it.blocks; ++j, ++n) {
+        const int s = n & 1;
+        const uint32_t ph = (n >> 1) & 1;
+        const bool seen = pr_seen_by_item(it, pr_block(it, j) + row);
+        // the packed K and V
+        const int slot_v = slot + 1 == kPrRaw ? 0 : slot + 1;
+        const uint32_t turn_v = slot + 1 == kPrRaw ? turn ^ 1 : turn;
+        const uint8_t *raw_k = sm + L::o_raw + slot * L::raw, *raw_v = sm + L::o_raw + slot_v * L::raw;
+        if (!attn_wait(bars.raw_full + 8 * slot, turn, abort, p.err)) break;
+        if (!attn_wait(bars.raw_full + 8 * slot_v, turn_v, abort, p.err)) break;
+        uint32_t kp[NJ], vp[NJ];
+        lds_words<NJ>(raw_k + o_par, kp);
+        lds_words<NJ>(raw_v + o_par, vp);
+        // the block's exponents
+        uint32_t mask = 0;
 #pragma unroll
-        for (int g = 0; g < NJ; g += 2) {
-          const uint32_t s2 = pack_f16x2(bf16_lo_f32(vp[g]) * up20, bf16_lo_f32(vp[g + 1]) * up20);
-          const uint32_t m2 = pack_f16x2(bf16_hi_f32(vp[g]) * up, bf16_hi_f32(vp[g + 1]) * up);
-#pragma unroll
-          for (int q = 0; q < 8; ++q)   // word (q NJ + g) / 2 of the row
-            *reinterpret_cast<uint4 *>(dst + pr_chunk(row, (q * NJ + g) / 2)) = pr_unpack(vc[(q * NJ + g) / 2], s2, m2);
+        for (int i = 0; i < NJ; ++i) {
+          if (!seen) kp[i] = vp[i] = 0;
+          if (((vp[i] >> 7) & 0xFF) == 0xFF || ((vp[i] >> 23) & 0xFF) == 0xFF) mask |= 1u << i, vp[i] = 0;
+          if (((kp[i] >> 7) & 0xFF) == 0xFF || ((kp[i] >> 23) & 0xFF) == 0xFF) mask |= 0x80u, kp[i] = 0;
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(bars.vfull + 8 * s);
+        const int ke = (int)__reduce_max_sync(0xffffffffu, (uint32_t)pr_exponent<NJ>(kp));
+        const int ve = (int)__reduce_max_sync(0xffffffffu, (uint32_t)pr_exponent<NJ>(vp)) |
+                       (__any_sync(0xffffffffu, mask != 0) ? 0x1000 : 0);
+        if (lane == 0) {
+          red[s * 4 + w4] = make_int2(ke, ve);
+          mbar_arrive(bars.vote);
+        }
+        if (!attn_wait(bars.vote, n & 1, abort, p.err)) break;
+        int k_exp = 0, bad = 0;
+        if (j == 0) v_exp = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int2 e = red[s * 4 + i];
+          k_exp = max(k_exp, e.x);
+          v_exp = max(v_exp, e.y & 0xFFF);
+          bad |= e.y >> 12;
+        }
+        const int fk = pr_shift(k_exp), fv = pr_shift(v_exp);
+        // K, then V: four words of codes at a time, each with its {scale, min}
+#pragma unroll 1
+        for (int v = 0; v < 2; ++v) {
+          if (!attn_wait((v ? bars.v_empty : bars.k_empty) + 8 * s, ph ^ 1, abort, p.err)) break;
+          if (!v) {
+            if (bad) poison[(n % kPrInfo) * kPrRows + row] = (uint8_t)mask;
+            if (row == 0) info[n % kPrInfo] = make_int4(fk, fv, bad, 0);
+          }
+          const float up = pow2f(v ? fv : fk), up20 = up * 0x1p20f;
+          uint32_t s2[4], m2[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            // a K word is of group w % NJ; a V word holds groups 2 (w % (NJ / 2)) and the next
+            const uint32_t lo = v ? vp[2 * (w % (NJ / 2))] : kp[w % NJ], hi = v ? vp[2 * (w % (NJ / 2)) + 1] : kp[w % NJ];
+            s2[w] = pack_f16x2(bf16_lo_f32(lo) * up20, bf16_lo_f32(hi) * up20);
+            m2[w] = pack_f16x2(bf16_hi_f32(lo) * up, bf16_hi_f32(hi) * up);
+          }
+          const uint8_t *src = (v ? raw_v : raw_k) + o_codes;
+          uint8_t *dst = sm + (v ? L::o_v : L::o_k) + s * L::tile + row * 128;
+#pragma unroll 1
+          for (int i0 = 0; i0 < NJ; ++i0) {
+            const int i = NJ == 4 ? i0 ^ ((row >> 1) & 3) : i0 ^ ((row >> 2) & 1);   // rows of eight lanes at eight banks
+            uint32_t w[4];
+            lds_words<4>(src + 16 * i, w);
+            // chunks 4 i .. 4 i + 3 of the row
+            uint8_t *half = dst + (i >> 1) * (kPrRows * 128);
+            const uint32_t x = (uint32_t)((4 * i ^ row) & 7) << 4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4 *>(half + (x ^ (e << 4))) = pr_unpack(w[e], s2[e], m2[e]);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          mbar_arrive((v ? bars.v_full : bars.k_full) + 8 * s);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars.raw_empty + 8 * (v ? slot_v : slot));
+        }
+        slot = slot_v + 1 == kPrRaw ? 0 : slot_v + 1;
+        turn = slot_v + 1 == kPrRaw ? turn_v ^ 1 : turn_v;
       }
-      if (j + 1 < it.blocks) fetch(j + 1);
     }
-  } else if (warp == 12 && it.blocks && lane == 0) {
-    // ------------------------------------------------------------ products --
-    constexpr uint32_t id_s = pr_idesc(kPrRows, false), id_o = pr_idesc(D, true);
-    constexpr uint32_t kBlock = kPrRows * 128;           // a 64-value column block of a tile
-    const uint32_t q_at = smem_addr(sm + L::o_q), k_at = smem_addr(sm + L::o_k), v_at = smem_addr(sm + L::o_v);
-    int at[2] = {0, 0};                                   // block of a tile's next product
-    bool scored[2] = {false, false};                      // its S is issued
-    bool q_ready = false;
-    uint64_t t_last = global_timer_ns();
-    while (at[0] < it.blocks || (tiles == 2 && at[1] < it.blocks)) {
-      bool any = false;
-      if (!q_ready) q_ready = mbar_try_wait(bars.q, 0);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int j = at[t], s = j & 1;
-        if (t >= tiles || j >= it.blocks || !q_ready) continue;
-        const uint32_t ph = (j >> 1) & 1;
-        if (!scored[t]) {
-          if (!mbar_try_wait(bars.kfull + 8 * s, ph) || (j > 0 && !mbar_try_wait(bars.odone + 8 * t, (j - 1) & 1))) continue;
-          pr_fence_after();
+  } else {
+    if (warp == 13) {
+      // ----------------------------------------------------------- items --
+      const int total = prefix[(p.b.n_seqs + 31) / 32];
+#pragma unroll 1
+      for (int k = 0;; ++k) {
+        if (!attn_wait(bars.item_empty + 8 * (k & 1), ((k >> 1) & 1) ^ 1, abort, p.err)) break;
+        const int i = pr_turn(k);
+        PrItem it;
+        it.b = -1;
+        if (i < total) it = pr_item(p, prefix, i, lane);
+        if (lane == 0) {
+          *reinterpret_cast<PrItem *>(sm + L::o_item + 64 * (k & 1)) = it;
+          mbar_arrive(bars.item_full + 8 * (k & 1));
+        }
+        __syncwarp();
+        if (i >= total) break;
+      }
+    } else if (warp == 14) {
+      // ------------------------------------------------- packed K and V --
+      int slot = 0;
+      uint32_t turn = 0;
+      const uint32_t part = p.g.head_bytes / 2;           // K or V of a page
+      bool ok = true;
+#pragma unroll 1
+      for (int k = 0; ok; item_done(k), ++k) {
+        ok = attn_wait(bars.item_full + 8 * (k & 1), (k >> 1) & 1, abort, p.err);
+        if (!ok) break;
+        const PrItem &it = *reinterpret_cast<const PrItem *>(sm + L::o_item + 64 * (k & 1));
+        if (it.b < 0) break;
+#pragma unroll 1
+        for (int j = 0; j < it.blocks && ok; ++j) {
+          // lane l: page l of the block, unless nobody sees its tokens
+          const int t = pr_block(it, j) + (lane << p.g.log2_page);
+          const uint8_t *src = nullptr;
+          if (lane < kPrRows >> p.g.log2_page && t < it.len && (t + p.g.page > it.lo || t < it.sinks))
+            src = kv_head_block(p.g, p.b, it.b, t, it.head, p.err);
+          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, src != nullptr)) * part;
+#pragma unroll 1
+          for (int v = 0; v < 2; ++v) {
+            ok = attn_wait(bars.raw_empty + 8 * slot, turn ^ 1, abort, p.err);
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(bars.raw_full + 8 * slot, bytes);
+            __syncwarp();
+            if (src)
+              bulk_copy_g2s_plain(smem_addr(sm + L::o_raw + slot * L::raw) + lane * part, src + (v ? part : 0), part,
+                                  bars.raw_full + 8 * slot);
+            if (++slot == kPrRaw) slot = 0, turn ^= 1;
+          }
+        }
+      }
+      // copies in flight land before the CTA leaves (their slots' last phases, each with a limit)
+      for (int i = 0; i < kPrRaw; ++i) {
+        const int w = (slot + i) % kPrRaw;
+        mbar_wait_bounded_warp(bars.raw_full + 8 * w, w < slot ? turn : turn ^ 1);
+      }
+    } else if (warp == 12) {
+      // -------------------------------------------------------- products --
+      constexpr uint32_t id_s = pr_idesc(kPrRows, false), id_o = pr_idesc(D, true);
+      constexpr uint32_t kBlock = kPrRows * 128;          // a 64-value column block of a tile
+      const uint32_t q_at = smem_addr(sm + L::o_q), k_at = smem_addr(sm + L::o_k), v_at = smem_addr(sm + L::o_v);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      // By tile (bit t): parity of the scores issued and of the items begun, whether there were any scores / two items.
+      uint32_t made = 0, made_any = 0, taken = 0, taken_any = 0, taken_two = 0;
+      // scores of block n (of all) for tile t; first / last block of its item; frees: the stage's last use
+      auto scores = [&](int t, int n, bool first, bool last, bool frees) {
+        const int s = n & 1;
+        if (first && !attn_wait(bars.q_full + 8 * t, (taken >> t) & 1, abort, p.err)) return false;
+        if (!attn_wait(bars.k_full + 8 * s, (n >> 1) & 1, abort, p.err)) return false;
+        // S and P share their columns: the product that reads P comes to its end first
+        if ((made_any >> t) & 1 && !attn_wait(bars.o_done + 8 * t, ((made >> t) & 1) ^ 1, abort, p.err)) return false;
+        pr_fence_after();
+        if (pr_elect()) {
+          const uint32_t d = tm + L::s_col + t * kPrRows;
+          const uint32_t da = pr_desc(q_at + t * L::tile, 16), db = pr_desc(k_at + s * L::tile, 16);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k >> 2) * kBlock + (k & 3) * 32;
-            pr_mma_ss(tmem + L::s_col + t * kPrRows, pr_desc(q_at + t * L::tile + off, 16), pr_desc(k_at + s * L::tile + off, 16),
-                      id_s, k > 0);
+            const uint32_t off = ((k >> 2) * kBlock + (k & 3) * 32) >> 4;
+            pr_mma_ss(d, da + off, db + off, id_s, k > 0);
           }
-          pr_commit(bars.sfull + 8 * t);
-          pr_commit(bars.kempty + 8 * s);
-          scored[t] = true;
-        } else {
-          if (!mbar_try_wait(bars.pfull + 8 * t, j & 1) || !mbar_try_wait(bars.vfull + 8 * s, ph)) continue;
-          pr_fence_after();
-#pragma unroll
-          for (int k = 0; k < kPrRows / 16; ++k)
-            pr_mma_ts(tmem + L::o_col + t * D, tmem + L::s_col + t * kPrRows + 8 * k,
-                      pr_desc(v_at + s * L::tile + k * 2048, kBlock), id_o, j > 0 || k > 0);
-          pr_commit(bars.odone + 8 * t);
-          pr_commit(bars.vempty + 8 * s);
-          scored[t] = false;
-          ++at[t];
+          pr_commit(bars.s_full + 8 * t);
+          if (frees) pr_commit(bars.k_empty + 8 * s);
+          if (last) pr_commit(bars.q_empty + 8 * t);
         }
-        any = true;
+        __syncwarp();
+        if (first) taken_two |= taken_any & (1u << t), taken_any |= 1u << t, taken ^= 1u << t;
+        made_any |= 1u << t, made ^= 1u << t;
+        return true;
+      };
+      auto values = [&](int t, int n, bool first, bool frees) {
+        const int s = n & 1;
+        if (!attn_wait(bars.v_full + 8 * s, (n >> 1) & 1, abort, p.err)) return false;
+        // the tile's previous results have been read
+        if (first && (taken_two >> t) & 1 && !attn_wait(bars.o_empty + 8 * t, (taken >> t) & 1, abort, p.err)) return false;
+        if (!attn_wait(bars.p_full + 8 * t, ((made >> t) & 1) ^ 1, abort, p.err)) return false;
+        pr_fence_after();
+        if (pr_elect()) {
+          const uint32_t d = tm + L::o_col + t * D, at = tm + L::s_col + t * kPrRows;
+          const uint32_t db = pr_desc(v_at + s * L::tile, kBlock);
+#pragma unroll
+          for (int k = 0; k < kPrRows / 16; ++k) pr_mma_ts(d, at + 8 * k, db + k * (2048 >> 4), id_o, !first || k > 0);
+          pr_commit(bars.o_done + 8 * t);
+          if (frees) pr_commit(bars.v_empty + 8 * s);
+        }
+        __syncwarp();
+        return true;
+      };
+      int k = 0, n = 0, tiles = 0, blocks = 0, next_tiles = 0, next_blocks = 0;
+      auto fetch = [&](int &to_tiles, int &to_blocks) {   // the next item that has blocks
+        for (;; item_done(k), ++k) {
+          if (!attn_wait(bars.item_full + 8 * (k & 1), (k >> 1) & 1, abort, p.err)) return false;
+          const PrItem *it = reinterpret_cast<const PrItem *>(sm + L::o_item + 64 * (k & 1));
+          if (it->b < 0) return false;
+          to_tiles = it->tiles;
+          to_blocks = it->blocks;
+          if (to_blocks) return true;
+        }
+      };
+      bool have = fetch(tiles, blocks), ok = true;
+#pragma unroll 1
+      for (int t = 0; t < 2; ++t)
+        if (have && t < tiles && ok) ok = scores(t, 0, true, blocks == 1, t == tiles - 1);
+      while (have && ok) {
+        bool more = false;
+#pragma unroll 1
+        for (int j = 0; j < blocks && ok; ++j, ++n) {
+          const bool last = j + 1 == blocks;
+          if (last) {
+            item_done(k);
+            ++k;
+            more = fetch(next_tiles, next_blocks);
+          }
+#pragma unroll 1
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (t < tiles) ok = values(t, n, j == 0, t == tiles - 1);
+            const int nt = last ? (more ? next_tiles : 0) : tiles;
+            if (ok && t < nt) ok = scores(t, n + 1, last, last ? next_blocks == 1 : j + 2 == blocks, t == nt - 1);
+          }
+        }
+        have = more;
+        tiles = next_tiles;
+        blocks = next_blocks;
       }
-      const uint64_t now = global_timer_ns();
-      if (any) t_last = now;
-      else if (*abort) break;
-      else if (now - t_last > 2000000000ull) {
-        *abort = 1;
-        atomicCAS(p.err, 0, kErrWaitTimeout);
-        break;
-      }
+      if (pr_elect()) pr_commit(bars.drain);              // whatever was issued has ended before the memory is given back
+      mbar_wait_bounded_warp(bars.drain, 0);
     }
-    pr_commit(bars.drain);                                // whatever was issued has ended before the memory is given back
-    mbar_wait_bounded(bars.drain, 0);
   }
   __syncwarp();
   pr_fence_before();
   __syncthreads();
-  if (warp == 12 && it.blocks) {
+  if (warp == 12) {
     pr_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPrTmemCols));
   }
@@ -611,7 +829,7 @@ static int prompt_launch(rc_ctx *ctx, const AttnParams &a, cudaStream_t s) {
     if (ctx->device < 64) ready[ctx->device].store(true, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)items);
+  cfg.gridDim = dim3((unsigned)(items < ctx->sm_count ? items : ctx->sm_count));
   cfg.blockDim = dim3(kPrThreads);
   cfg.dynamicSmemBytes = L::bytes;
   cfg.stream = s;
