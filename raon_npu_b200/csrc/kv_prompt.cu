@@ -4,18 +4,20 @@
 // Rows are (query, head of the kv head's group): 128 of them a tile, two tiles
 // a CTA, so a dequantised block of 128 tokens serves 256 rows.  Per block:
 //   S_t = Q_t K^T            f16 x f16 -> f32 in tensor memory
-//   P_t = 2^(c S_t - ref)    one thread a row; f16, written over S_t
+//   P_t = 2^(c S_t - ref)    one thread a row; f16, to tensor memory
 //   O_t = O_t + P_t V        P from tensor memory, f32 accumulators there
 // Roles: eight softmax warps (a tile for four of them, one thread a row; they
-// also write the results), four warps that make Q, K and V f16 in shared memory,
-// one that copies the packed K and V in, one that issues the products, one that
-// finds the items.  A tile's next scores follow its values of this block, so a
-// tile's softmax has the time of the other's products.  CTAs are persistent and
-// every role goes straight from one item to the next, so the next item's query
-// rows and blocks come in while the last one's results go out.
-// The roles' loops are rolled and short on purpose: with the scores of a row in
-// registers and everything unrolled, the roles together outgrew the instruction
-// cache and each of them, the issuing warp first, ran at the speed of its misses.
+// also write the results), four warps that make K f16 in shared memory and four
+// for V (and Q, a tile each), one that copies the packed K and V in, one that
+// issues the products, one that finds the items.  A row's scores are read into
+// registers at once (setmaxnreg takes them from the other roles), which frees the
+// tensor memory of S for the other tile's scores: the two tiles share one S and
+// have a P each, and a tile's next scores are there when its softmax comes for
+// them.  CTAs are persistent and every role goes straight from one item to the
+// next, so the next item's query rows and blocks come in while the last one's
+// results go out.  The loops of the other roles are rolled and short on purpose:
+// together with a larger text they outgrew the instruction cache, and each of
+// them, the issuing warp first, ran at the speed of its misses.
 //
 // Numbers: K, V, Q and P are f16 (11 bits; one rounding each).  Q is scaled by
 // a power of two per row, K per block and V by a power of two that follows the
@@ -34,9 +36,12 @@
 namespace rc {
 
 constexpr int kPrRows = 128;                         // rows of a tile, tokens of a block
-constexpr int kPrThreads = 512;
+constexpr int kPrThreads = 640;
+// Registers: the softmax warpgroups get what the others leave of 640 x 96.
+constexpr int kPrRegsSoftmax = 160, kPrRegsMake = 56, kPrRegsIssue = 48;
+static_assert(2 * kPrRegsSoftmax + 2 * kPrRegsMake + kPrRegsIssue == 5 * 96, "setmaxnreg draws on the launch's registers");
 constexpr int kPrInfo = 4;                           // blocks whose exponents are kept
-constexpr int kPrRaw = 3;                            // packed K or V blocks on their way in
+constexpr int kPrRaw = 3;                            // packed K and V blocks (by turns) on their way in
 constexpr uint32_t kPrTmemCols = 512;
 // The rows of an item and the blocks of tokens they see.
 struct PrItem {
@@ -51,19 +56,19 @@ struct PrLayout {
   static constexpr int D = 32 * NJ;
   static constexpr int tile = kPrRows * D * 2;
   static constexpr int o_q = 0, o_k = 2 * tile, o_v = o_k + 2 * tile;
-  static constexpr int o_poison = o_v + 2 * tile;                 // [kPrInfo][128] group masks of NaN values, bit 7: NaN key
-  static constexpr int o_info = o_poison + kPrInfo * kPrRows;     // [kPrInfo]{K exponent, V exponent, poisoned, -}
-  static constexpr int o_red = o_info + kPrInfo * 16;             // [2][4 warps]{K, V}
+  static constexpr int o_poison = o_v + 2 * tile;                 // [kPrInfo][K, V][128] groups that hold NaN (V), bit 7 for any of K
+  static constexpr int o_info = o_poison + 2 * kPrInfo * kPrRows; // [kPrInfo]{exponent, poisoned} of K and of V
+  static constexpr int o_red = o_info + kPrInfo * 16;             // [K, V][2][4 warps] exponents
   static constexpr int o_crow = o_red + 64;                       // [2 items][256] score scales, NaN for a row that is
   static constexpr int o_item = o_crow + 2 * 2 * kPrRows * 4;     // [2] items
   static constexpr int o_bar = o_item + 2 * 64;
-  static constexpr int n_bars = 32;
+  static constexpr int n_bars = 33 + 2 * kPrRaw;
   static constexpr int o_misc = o_bar + 8 * n_bars;               // tensor memory address, abort word
   static constexpr int o_prefix = o_misc + 16;                    // [n_seqs / 32 + 1] items of the sequences before
   static constexpr int o_raw = (o_prefix + (kKvMaxSeqs / 32 + 1) * 4 + 127) / 128 * 128;
   static constexpr int raw = kPrRows * D * 5 / 8;                 // packed K or V of a block
-  static constexpr int bytes = o_raw + kPrRaw * raw + 1024;       // and the alignment
-  static constexpr uint32_t s_col = 0, o_col = 2 * kPrRows;       // tensor memory: S0 S1 O0 O1
+  static constexpr int bytes = o_raw + kPrRaw * raw;
+  static constexpr uint32_t s_col = 0, p_col = kPrRows, o_col = 2 * kPrRows;   // tensor memory: S, P0 P1, O0 O1
 };
 static_assert(sizeof(PrItem) <= 64, "an item's slot");
 static_assert(PrLayout<4>::bytes <= kGemvSmemLimit, "shared memory of an SM");
@@ -224,7 +229,7 @@ __device__ __forceinline__ uint32_t pr_chunk(int r, int c) {
 }
 
 struct PrBars {
-  uint32_t item_full, item_empty, q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_empty, drain, vote, raw_full, raw_empty;
+  uint32_t item_full, item_empty, q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_empty, drain, vote, s_free, v_info, raw_full, raw_empty;
 };
 
 // Of columns 32 k .. 32 k + 31, those a row sees: column <= c_hi, and > c_lo or < c_sink.
@@ -236,6 +241,14 @@ __device__ __forceinline__ uint32_t pr_seen(int k, int c_hi, int c_lo, int c_sin
   return upto & (past | first);
 }
 
+__device__ __forceinline__ void pr_touch(uint32_t (&v)[32]) {   // nothing uses v before this point
+  asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]),
+                 "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]),
+                 "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]),
+                 "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                 "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
+                 "+r"(v[30]), "+r"(v[31]));
+}
 __device__ __forceinline__ void pr_scale8(uint32_t addr, float by) {
   uint32_t v[8];
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -271,65 +284,20 @@ __device__ __forceinline__ uint64_t pr_add2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// Largest score of this thread's row (in the product's units).
-template <bool MASKED>
-__device__ __forceinline__ float pr_top(uint32_t s_at, int c_hi, int c_lo, int c_sink) {
-  float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-  for (int k = 0; k < 4; ++k) {
-    uint32_t v[32];
-    pr_ld32(s_at + 32 * k, v);
-    const uint32_t seen = MASKED ? pr_seen(k, c_hi, c_lo, c_sink) : ~0u;
-    pr_wait_ld(v);
-#pragma unroll
-    for (int e = 0; e < 32; e += 2) {
-      const float x0 = MASKED && !(seen >> e & 1) ? -INFINITY : __uint_as_float(v[e]);
-      const float x1 = MASKED && !(seen >> (e + 1) & 1) ? -INFINITY : __uint_as_float(v[e + 1]);
-      a[(e >> 1) & 3] = fmaxf(fmaxf(a[(e >> 1) & 3], x0), x1);
-    }
-  }
-  return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
-}
-
-// Weights 2^(c S + minus) of this thread's row, f16, over the scores; returns their sum.
-template <bool MASKED>
-__device__ __forceinline__ float pr_weights(uint32_t s_at, float c, float minus, int c_hi, int c_lo, int c_sink) {
-  const uint64_t c2 = pr_pair(c, c), m2 = pr_pair(minus, minus);
-  uint64_t sum[2] = {0, 0};
-#pragma unroll 1
-  for (int k = 0; k < 4; ++k) {
-    uint32_t v[32], w[16];
-    pr_ld32(s_at + 32 * k, v);
-    const uint32_t seen = MASKED ? pr_seen(k, c_hi, c_lo, c_sink) : ~0u;
-    pr_wait_ld(v);
-#pragma unroll
-    for (int e = 0; e < 32; e += 2) {
-      float x0, x1;
-      pr_split(pr_fma2(pr_pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), c2, m2), x0, x1);
-      if (MASKED && !(seen >> e & 1)) x0 = -INFINITY;
-      if (MASKED && !(seen >> (e + 1) & 1)) x1 = -INFINITY;
-      x0 = ex2(x0);
-      x1 = ex2(x1);
-      sum[(e >> 1) & 1] = pr_add2(sum[(e >> 1) & 1], pr_pair(x0, x1));
-      w[e / 2] = pack_f16x2(x0, x1);
-    }
-    pr_st16(s_at + 16 * k, w);
-  }
-  float a, b;
-  pr_split(pr_add2(sum[0], sum[1]), a, b);
-  return a + b;
-}
-
 template <int NJ>
 __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __grid_constant__ AttnParams p) {
   using L = PrLayout<NJ>;
   constexpr int D = L::D;
-  extern __shared__ uint8_t pr_raw[];
-  uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pr_raw) + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t pr_raw[];
+  uint8_t *sm = pr_raw;
+  if (smem_addr(sm) & 1023) {   // the swizzled tiles start on their pattern; there is no room to move them
+    atomicCAS(p.err, 0, kErrWaitTimeout);
+    return;
+  }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t bar0 = smem_addr(sm + L::o_bar);
   const PrBars bars{bar0,       bar0 + 16,  bar0 + 32,  bar0 + 48,  bar0 + 64,  bar0 + 80, bar0 + 96,
-                    bar0 + 112, bar0 + 128, bar0 + 144, bar0 + 160, bar0 + 176, bar0 + 192, bar0 + 200, bar0 + 208, bar0 + 232};
+                    bar0 + 112, bar0 + 128, bar0 + 144, bar0 + 160, bar0 + 176, bar0 + 192, bar0 + 208, bar0 + 224, bar0 + 232, bar0 + 264, bar0 + 264 + 8 * kPrRaw};
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + L::o_misc);
   volatile int *abort = reinterpret_cast<volatile int *>(sm + L::o_misc + 4);
   int4 *info = reinterpret_cast<int4 *>(sm + L::o_info);
@@ -340,7 +308,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
     *abort = 0;
     for (int s = 0; s < 2; ++s) {
       mbar_init(bars.item_full + 8 * s, 1);
-      mbar_init(bars.item_empty + 8 * s, 14);            // eight softmax warps, four that make operands, copies, products
+      mbar_init(bars.item_empty + 8 * s, 19);            // softmax, operands, copies, scores, values
       mbar_init(bars.q_full + 8 * s, kPrRows);
       mbar_init(bars.q_empty + 8 * s, 1);
       mbar_init(bars.k_full + 8 * s, kPrRows);
@@ -353,7 +321,11 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
       mbar_init(bars.o_empty + 8 * s, 4);
     }
     mbar_init(bars.drain, 1);
+    mbar_init(bars.drain + 8, 1);
     mbar_init(bars.vote, 4);
+    mbar_init(bars.vote + 8, 4);
+    mbar_init(bars.s_free, 4);
+    for (int s = 0; s < kPrInfo; ++s) mbar_init(bars.v_info + 8 * s, 4);
     for (int s = 0; s < kPrRaw; ++s) {
       mbar_init(bars.raw_full + 8 * s, 1);
       mbar_init(bars.raw_empty + 8 * s, 4);
@@ -375,7 +347,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
     prefix[0] = 0;
 #pragma unroll 1
     for (int g = 0; g < (p.b.n_seqs + 31) / 32; ++g) prefix[g + 1] += prefix[g];
-  } else if (warp == 12) {
+  } else if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
                  "r"(kPrTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -391,9 +363,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
 
   if (warp < 8) {
     // ------------------------------------------------------------- softmax --
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPrRegsSoftmax));
     const int t = warp >> 2, row = tid & (kPrRows - 1);
     const uint32_t lane_at = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-    const uint32_t s_at = lane_at + L::s_col + t * kPrRows, o_at = lane_at + L::o_col + t * D;
+    const uint32_t s_at = lane_at + L::s_col, p_at = lane_at + L::p_col + t * (kPrRows / 2), o_at = lane_at + L::o_col + t * D;
     const uint32_t bar_s = bars.s_full + 8 * t, bar_p = bars.p_full + 8 * t, bar_o = bars.o_done + 8 * t;
     int n = 0, done = 0;                                  // blocks of all items so far; this tile's
 #pragma unroll 1
@@ -421,16 +394,48 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           ok = attn_wait(bar_s, done & 1, abort, p.err);
           if (!ok) break;
           pr_fence_after();
+          uint32_t v[4][32];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pr_ld32(s_at + 32 * i, v[i]);
           if (j == 0) {
             c_row = crow[(k & 1) * 2 * kPrRows + t * kPrRows + row];
             if (c_row != c_row) c_row = 0.f, nan_groups = (1u << NJ) - 1u;
           }
+          ok = attn_wait(bars.v_info + 8 * ((n + j) % kPrInfo), (n + j) / kPrInfo & 1, abort, p.err);
+          if (!ok) break;
           const int4 f = info[(n + j) % kPrInfo];
-          const float c = c_row * pow2f(-f.x);
+          const float c = fmaxf(c_row * pow2f(-f.x), 0x1p-126f);   // above 0: a hidden score is -Inf
           const int c_hi = pos - t0, c_lo = p.window > 0 ? c_hi - p.window : INT_MIN, c_sink = p.sinks - t0;
-          const float top = masked ? pr_top<true>(s_at, c_hi, c_lo, c_sink) : pr_top<false>(s_at, 0, 0, 0);
-          const float x_top = top == -INFINITY ? -INFINITY : top * c;
-          if (__any_sync(0xffffffffu, x_top > ref + kAttnSlack || f.y != fv)) {
+          pr_wait_ld(v[0]);
+          pr_touch(v[1]);
+          pr_touch(v[2]);
+          pr_touch(v[3]);
+          pr_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars.s_free);
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t seen = pr_seen(i, c_hi, c_lo, c_sink);
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!(seen >> e & 1)) v[i][e] = 0xFF800000u;
+            }
+          }
+          float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+              top4[(e >> 1) & 3] = fmaxf(fmaxf(top4[(e >> 1) & 3], __uint_as_float(v[i][e])), __uint_as_float(v[i][e + 1]));
+          const float x_top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * c;
+          // the tile's last values are done: P may be written, O changed
+          if (done > 0) {
+            ok = attn_wait(bar_o, (done - 1) & 1, abort, p.err);
+            if (!ok) break;
+            pr_fence_after();
+          }
+          if (__any_sync(0xffffffffu, x_top > ref + kAttnSlack || f.z != fv)) {
             float by = 1.f;
             if (x_top > ref + kAttnSlack) {
               by = exp2f(ref - x_top);
@@ -438,24 +443,39 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
             }
             l *= by;
             if (j > 0) {
-              by *= pow2f(max(f.y - fv, -126));
-              ok = attn_wait(bar_o, (done - 1) & 1, abort, p.err);
-              if (!ok) break;
-              pr_fence_after();
+              by *= pow2f(max(f.z - fv, -126));
 #pragma unroll 1
               for (int i = 0; i < D / 8; ++i) pr_scale8(o_at + 8 * i, by);
             }
-            fv = f.y;
+            fv = f.z;
           }
           const float minus = ref == -INFINITY ? 0.f : kAttnLift - ref;
-          l += masked ? pr_weights<true>(s_at, c, minus, c_hi, c_lo, c_sink) : pr_weights<false>(s_at, c, minus, 0, 0, 0);
-          if (f.z) {
+          const uint64_t c2 = pr_pair(c, c), m2 = pr_pair(minus, minus);
+          uint64_t sum[2] = {0, 0};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float x0, x1;
+              pr_split(pr_fma2(pr_pair(__uint_as_float(v[i][e]), __uint_as_float(v[i][e + 1])), c2, m2), x0, x1);
+              x0 = ex2(x0);
+              x1 = ex2(x1);
+              sum[(e >> 1) & 1] = pr_add2(sum[(e >> 1) & 1], pr_pair(x0, x1));
+              w[e / 2] = pack_f16x2(x0, x1);
+            }
+            pr_st16(p_at + 16 * i, w);
+          }
+          float s0, s1;
+          pr_split(pr_add2(sum[0], sum[1]), s0, s1);
+          l += s0 + s1;
+          if (f.y | f.w) {
             // groups of this block that hold NaN, in tokens that this row sees
 #pragma unroll 1
             for (int col = 0; col < kPrRows; ++col) {
               const bool see = col <= c_hi && (col > c_lo || col < c_sink);
-              const uint32_t m = poison[((n + j) % kPrInfo) * kPrRows + col];
-              if (see) nan_groups |= m & 0x80 ? (1u << NJ) - 1u : m;
+              const uint8_t *m = poison + (n + j) % kPrInfo * 2 * kPrRows + col;
+              if (see) nan_groups |= m[0] ? (1u << NJ) - 1u : m[kPrRows];
             }
           }
           pr_wait_st();
@@ -513,18 +533,20 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
       n += blocks;
       item_done(k);
     }
-  } else if (warp < 12) {
+  } else if (warp < 16) {
     // -------------------------------------------------- operands as f16 --
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrRegsMake));
+    const int kv = (warp - 8) >> 2;                       // 0: K and tile 0's Q; 1: V and tile 1's Q
     const int row = tid & (kPrRows - 1), w4 = warp & 3;
-    int2 *red = reinterpret_cast<int2 *>(sm + L::o_red);
+    int *red = reinterpret_cast<int *>(sm + L::o_red) + 8 * kv;
+    const uint32_t bar_full = (kv ? bars.v_full : bars.k_full), bar_empty = (kv ? bars.v_empty : bars.k_empty);
+
     // this row's codes and params within a packed block: the pages' parts one after the other
     const uint32_t sub = (uint32_t)(row >> p.g.log2_page) * (p.g.head_bytes / 2);
     const uint32_t o_codes = sub + (row & (p.g.page - 1)) * (D / 2);
     const uint32_t o_par = sub + p.g.kp_off + (row & (p.g.page - 1)) * (NJ * 4);
-    int n = 0, uses0 = 0, uses1 = 0;                      // blocks so far; items of each tile so far
-    int slot = 0;                                         // of the packed blocks
-    uint32_t turn = 0;
-    int v_exp = 0;
+    int n = 0, uses = 0;                                  // blocks so far; items of the tile so far
+    int exp = 0;
 #pragma unroll 1
     for (int k = 0;; item_done(k), ++k) {
       if (!attn_wait(bars.item_full + 8 * (k & 1), (k >> 1) & 1, abort, p.err)) break;
@@ -532,12 +554,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
       if (it.b < 0) break;
       if (it.blocks == 0) continue;
       // the item's query rows, 4 NJ lanes a row
-#pragma unroll 1
-      for (int t = 0; t < it.tiles; ++t) {
-        const bool free = attn_wait(bars.q_empty + 8 * t, ((t ? uses1 : uses0) & 1) ^ 1, abort, p.err);
-        if (t) ++uses1;
-        else ++uses0;
-        if (!free) continue;
+      const int t = kv;
+      if (t < it.tiles && attn_wait(bars.q_empty + 8 * t, (uses++ & 1) ^ 1, abort, p.err)) {
         constexpr int kLanes = 4 * NJ, kAtOnce = 4;
         const int i = row % kLanes;                       // dims 8i .. 8i+7 = 32j + 8q ..: chunk q * NJ + j
 #pragma unroll 1
@@ -583,85 +601,76 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
 
 #pragma unroll 1
       for (int j = 0; j < it.blocks; ++j, ++n) {
-        const int s = n & 1;
-        const uint32_t ph = (n >> 1) & 1;
+        const int s = n & 1, slot = (2 * n + kv) % kPrRaw;
+        const uint8_t *raw = sm + L::o_raw + slot * L::raw;
         const bool seen = pr_seen_by_item(it, pr_block(it, j) + row);
-        // the packed K and V
-        const int slot_v = slot + 1 == kPrRaw ? 0 : slot + 1;
-        const uint32_t turn_v = slot + 1 == kPrRaw ? turn ^ 1 : turn;
-        const uint8_t *raw_k = sm + L::o_raw + slot * L::raw, *raw_v = sm + L::o_raw + slot_v * L::raw;
-        if (!attn_wait(bars.raw_full + 8 * slot, turn, abort, p.err)) break;
-        if (!attn_wait(bars.raw_full + 8 * slot_v, turn_v, abort, p.err)) break;
-        uint32_t kp[NJ], vp[NJ];
-        lds_words<NJ>(raw_k + o_par, kp);
-        lds_words<NJ>(raw_v + o_par, vp);
-        // the block's exponents
+        if (!attn_wait(bars.raw_full + 8 * slot, (2 * n + kv) / kPrRaw & 1, abort, p.err)) break;
+        uint32_t par[NJ];
+        lds_words<NJ>(raw + o_par, par);
+        // the block's exponents; a NaN group is zero and told to the rows that see it
         uint32_t mask = 0;
 #pragma unroll
         for (int i = 0; i < NJ; ++i) {
-          if (!seen) kp[i] = vp[i] = 0;
-          if (((vp[i] >> 7) & 0xFF) == 0xFF || ((vp[i] >> 23) & 0xFF) == 0xFF) mask |= 1u << i, vp[i] = 0;
-          if (((kp[i] >> 7) & 0xFF) == 0xFF || ((kp[i] >> 23) & 0xFF) == 0xFF) mask |= 0x80u, kp[i] = 0;
+          if (!seen) par[i] = 0;
+          if (((par[i] >> 7) & 0xFF) == 0xFF || ((par[i] >> 23) & 0xFF) == 0xFF) mask |= kv ? 1u << i : 0x80u, par[i] = 0;
         }
-        const int ke = (int)__reduce_max_sync(0xffffffffu, (uint32_t)pr_exponent<NJ>(kp));
-        const int ve = (int)__reduce_max_sync(0xffffffffu, (uint32_t)pr_exponent<NJ>(vp)) |
-                       (__any_sync(0xffffffffu, mask != 0) ? 0x1000 : 0);
+        const int e = (int)__reduce_max_sync(0xffffffffu, (uint32_t)pr_exponent<NJ>(par)) |
+                      (__any_sync(0xffffffffu, mask != 0) ? 0x1000 : 0);
         if (lane == 0) {
-          red[s * 4 + w4] = make_int2(ke, ve);
-          mbar_arrive(bars.vote);
+          red[s * 4 + w4] = e;
+          mbar_arrive(bars.vote + 8 * kv);
         }
-        if (!attn_wait(bars.vote, n & 1, abort, p.err)) break;
-        int k_exp = 0, bad = 0;
-        if (j == 0) v_exp = 0;
+        if (!attn_wait(bars.vote + 8 * kv, n & 1, abort, p.err)) break;
+        if (j == 0 || !kv) exp = 0;                       // V's follows the largest of the item, K's is the block's own
+        int bad = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int2 e = red[s * 4 + i];
-          k_exp = max(k_exp, e.x);
-          v_exp = max(v_exp, e.y & 0xFFF);
-          bad |= e.y >> 12;
+          exp = max(exp, red[s * 4 + i] & 0xFFF);
+          bad |= red[s * 4 + i] >> 12;
         }
-        const int fk = pr_shift(k_exp), fv = pr_shift(v_exp);
-        // K, then V: four words of codes at a time, each with its {scale, min}
-#pragma unroll 1
-        for (int v = 0; v < 2; ++v) {
-          if (!attn_wait((v ? bars.v_empty : bars.k_empty) + 8 * s, ph ^ 1, abort, p.err)) break;
-          if (!v) {
-            if (bad) poison[(n % kPrInfo) * kPrRows + row] = (uint8_t)mask;
-            if (row == 0) info[n % kPrInfo] = make_int4(fk, fv, bad, 0);
-          }
-          const float up = pow2f(v ? fv : fk), up20 = up * 0x1p20f;
-          uint32_t s2[4], m2[4];
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            // a K word is of group w % NJ; a V word holds groups 2 (w % (NJ / 2)) and the next
-            const uint32_t lo = v ? vp[2 * (w % (NJ / 2))] : kp[w % NJ], hi = v ? vp[2 * (w % (NJ / 2)) + 1] : kp[w % NJ];
-            s2[w] = pack_f16x2(bf16_lo_f32(lo) * up20, bf16_lo_f32(hi) * up20);
-            m2[w] = pack_f16x2(bf16_hi_f32(lo) * up, bf16_hi_f32(hi) * up);
-          }
-          const uint8_t *src = (v ? raw_v : raw_k) + o_codes;
-          uint8_t *dst = sm + (v ? L::o_v : L::o_k) + s * L::tile + row * 128;
-#pragma unroll 1
-          for (int i0 = 0; i0 < NJ; ++i0) {
-            const int i = NJ == 4 ? i0 ^ ((row >> 1) & 3) : i0 ^ ((row >> 2) & 1);   // rows of eight lanes at eight banks
-            uint32_t w[4];
-            lds_words<4>(src + 16 * i, w);
-            // chunks 4 i .. 4 i + 3 of the row
-            uint8_t *half = dst + (i >> 1) * (kPrRows * 128);
-            const uint32_t x = (uint32_t)((4 * i ^ row) & 7) << 4;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4 *>(half + (x ^ (e << 4))) = pr_unpack(w[e], s2[e], m2[e]);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          mbar_arrive((v ? bars.v_full : bars.k_full) + 8 * s);
+        const int f = pr_shift(exp);
+        auto tell = [&] {
+          poison[((n % kPrInfo) * 2 + kv) * kPrRows + row] = (uint8_t)mask;
+          if (row == 0) *(reinterpret_cast<int2 *>(info + n % kPrInfo) + kv) = make_int2(f, bad);
+        };
+        if (kv) {                                         // the softmax threads wait for V's exponent by itself
+          tell();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bars.raw_empty + 8 * (v ? slot_v : slot));
+          if (lane == 0) mbar_arrive(bars.v_info + 8 * (n % kPrInfo));
         }
-        slot = slot_v + 1 == kPrRaw ? 0 : slot_v + 1;
-        turn = slot_v + 1 == kPrRaw ? turn_v ^ 1 : turn_v;
+        if (!attn_wait(bar_empty + 8 * s, ((n >> 1) & 1) ^ 1, abort, p.err)) break;
+        if (!kv) tell();                                  // not before: block n - 4's may still be read
+        // four words of codes at a time, each with its {scale, min}
+        const float up = pow2f(f), up20 = up * 0x1p20f;
+        uint32_t s2[4], m2[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          // a K word is of group w % NJ; a V word holds groups 2 (w % (NJ / 2)) and the next
+          const uint32_t lo = kv ? par[2 * (w % (NJ / 2))] : par[w % NJ], hi = kv ? par[2 * (w % (NJ / 2)) + 1] : par[w % NJ];
+          s2[w] = pack_f16x2(bf16_lo_f32(lo) * up20, bf16_lo_f32(hi) * up20);
+          m2[w] = pack_f16x2(bf16_hi_f32(lo) * up, bf16_hi_f32(hi) * up);
+        }
+        uint8_t *dst = sm + (kv ? L::o_v : L::o_k) + s * L::tile + row * 128;
+#pragma unroll 1
+        for (int i0 = 0; i0 < NJ; ++i0) {
+          const int i = NJ == 4 ? i0 ^ ((row >> 1) & 3) : i0 ^ ((row >> 2) & 1);   // rows of eight lanes at eight banks
+          uint32_t w[4];
+          lds_words<4>(raw + o_codes + 16 * i, w);
+          // chunks 4 i .. 4 i + 3 of the row
+          uint8_t *half = dst + (i >> 1) * (kPrRows * 128);
+          const uint32_t x = (uint32_t)((4 * i ^ row) & 7) << 4;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4 *>(half + (x ^ (e << 4))) = pr_unpack(w[e], s2[e], m2[e]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(bar_full + 8 * s);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars.raw_empty + 8 * slot);
       }
     }
   } else {
-    if (warp == 13) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrRegsIssue));
+    if (warp == 17) {
       // ----------------------------------------------------------- items --
       const int total = prefix[(p.b.n_seqs + 31) / 32];
 #pragma unroll 1
@@ -678,11 +687,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
         __syncwarp();
         if (i >= total) break;
       }
-    } else if (warp == 14) {
+    } else if (warp == 18) {
       // ------------------------------------------------- packed K and V --
-      int slot = 0;
-      uint32_t turn = 0;
       const uint32_t part = p.g.head_bytes / 2;           // K or V of a page
+      int h = 0;                                          // packed blocks asked for: K, V, K, ...
       bool ok = true;
 #pragma unroll 1
       for (int k = 0; ok; item_done(k), ++k) {
@@ -699,118 +707,99 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
             src = kv_head_block(p.g, p.b, it.b, t, it.head, p.err);
           const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, src != nullptr)) * part;
 #pragma unroll 1
-          for (int v = 0; v < 2; ++v) {
-            ok = attn_wait(bars.raw_empty + 8 * slot, turn ^ 1, abort, p.err);
+          for (int v = 0; v < 2; ++v, ++h) {
+            const int slot = h % kPrRaw;
+            ok = attn_wait(bars.raw_empty + 8 * slot, (h / kPrRaw & 1) ^ 1, abort, p.err);
             if (!ok) break;
             if (lane == 0) mbar_arrive_expect_tx(bars.raw_full + 8 * slot, bytes);
             __syncwarp();
             if (src)
               bulk_copy_g2s_plain(smem_addr(sm + L::o_raw + slot * L::raw) + lane * part, src + (v ? part : 0), part,
                                   bars.raw_full + 8 * slot);
-            if (++slot == kPrRaw) slot = 0, turn ^= 1;
           }
         }
       }
-      // copies in flight land before the CTA leaves (their slots' last phases, each with a limit)
-      for (int i = 0; i < kPrRaw; ++i) {
-        const int w = (slot + i) % kPrRaw;
-        mbar_wait_bounded_warp(bars.raw_full + 8 * w, w < slot ? turn : turn ^ 1);
-      }
-    } else if (warp == 12) {
+      // copies in flight land before the CTA leaves: the last phase of each slot that had one, with a limit
+      for (int i = max(0, h - kPrRaw); i < h; ++i) mbar_wait_bounded_warp(bars.raw_full + 8 * (i % kPrRaw), i / kPrRaw & 1);
+    } else {
       // -------------------------------------------------------- products --
+      // Two warps: 16 issues the scores, 19 the values (one warp's instructions for both took longer than the products).
+      const bool is_v = warp == 19;
       constexpr uint32_t id_s = pr_idesc(kPrRows, false), id_o = pr_idesc(D, true);
       constexpr uint32_t kBlock = kPrRows * 128;          // a 64-value column block of a tile
       const uint32_t q_at = smem_addr(sm + L::o_q), k_at = smem_addr(sm + L::o_k), v_at = smem_addr(sm + L::o_v);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      // By tile (bit t): parity of the scores issued and of the items begun, whether there were any scores / two items.
-      uint32_t made = 0, made_any = 0, taken = 0, taken_any = 0, taken_two = 0;
-      // scores of block n (of all) for tile t; first / last block of its item; frees: the stage's last use
-      auto scores = [&](int t, int n, bool first, bool last, bool frees) {
-        const int s = n & 1;
-        if (first && !attn_wait(bars.q_full + 8 * t, (taken >> t) & 1, abort, p.err)) return false;
-        if (!attn_wait(bars.k_full + 8 * s, (n >> 1) & 1, abort, p.err)) return false;
-        // S and P share their columns: the product that reads P comes to its end first
-        if ((made_any >> t) & 1 && !attn_wait(bars.o_done + 8 * t, ((made >> t) & 1) ^ 1, abort, p.err)) return false;
-        pr_fence_after();
-        if (pr_elect()) {
-          const uint32_t d = tm + L::s_col + t * kPrRows;
-          const uint32_t da = pr_desc(q_at + t * L::tile, 16), db = pr_desc(k_at + s * L::tile, 16);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = ((k >> 2) * kBlock + (k & 3) * 32) >> 4;
-            pr_mma_ss(d, da + off, db + off, id_s, k > 0);
-          }
-          pr_commit(bars.s_full + 8 * t);
-          if (frees) pr_commit(bars.k_empty + 8 * s);
-          if (last) pr_commit(bars.q_empty + 8 * t);
-        }
-        __syncwarp();
-        if (first) taken_two |= taken_any & (1u << t), taken_any |= 1u << t, taken ^= 1u << t;
-        made_any |= 1u << t, made ^= 1u << t;
-        return true;
-      };
-      auto values = [&](int t, int n, bool first, bool frees) {
-        const int s = n & 1;
-        if (!attn_wait(bars.v_full + 8 * s, (n >> 1) & 1, abort, p.err)) return false;
-        // the tile's previous results have been read
-        if (first && (taken_two >> t) & 1 && !attn_wait(bars.o_empty + 8 * t, (taken >> t) & 1, abort, p.err)) return false;
-        if (!attn_wait(bars.p_full + 8 * t, ((made >> t) & 1) ^ 1, abort, p.err)) return false;
-        pr_fence_after();
-        if (pr_elect()) {
-          const uint32_t d = tm + L::o_col + t * D, at = tm + L::s_col + t * kPrRows;
-          const uint32_t db = pr_desc(v_at + s * L::tile, kBlock);
-#pragma unroll
-          for (int k = 0; k < kPrRows / 16; ++k) pr_mma_ts(d, at + 8 * k, db + k * (2048 >> 4), id_o, !first || k > 0);
-          pr_commit(bars.o_done + 8 * t);
-          if (frees) pr_commit(bars.v_empty + 8 * s);
-        }
-        __syncwarp();
-        return true;
-      };
-      int k = 0, n = 0, tiles = 0, blocks = 0, next_tiles = 0, next_blocks = 0;
-      auto fetch = [&](int &to_tiles, int &to_blocks) {   // the next item that has blocks
-        for (;; item_done(k), ++k) {
-          if (!attn_wait(bars.item_full + 8 * (k & 1), (k >> 1) & 1, abort, p.err)) return false;
-          const PrItem *it = reinterpret_cast<const PrItem *>(sm + L::o_item + 64 * (k & 1));
-          if (it->b < 0) return false;
-          to_tiles = it->tiles;
-          to_blocks = it->blocks;
-          if (to_blocks) return true;
-        }
-      };
-      bool have = fetch(tiles, blocks), ok = true;
+      uint32_t items = 0, any = 0, made = 0, valued = 0;  // by tile (bit t): parity of its items, whether there were any ...
+      int n = 0;                                          // ... of its values; scores of both tiles; blocks
+      bool ok = true;
 #pragma unroll 1
-      for (int t = 0; t < 2; ++t)
-        if (have && t < tiles && ok) ok = scores(t, 0, true, blocks == 1, t == tiles - 1);
-      while (have && ok) {
-        bool more = false;
+      for (int k = 0; ok; item_done(k), ++k) {
+        ok = attn_wait(bars.item_full + 8 * (k & 1), (k >> 1) & 1, abort, p.err);
+        if (!ok) break;
+        const PrItem *it = reinterpret_cast<const PrItem *>(sm + L::o_item + 64 * (k & 1));
+        if (it->b < 0) break;
+        const int tiles = it->tiles, blocks = it->blocks;
 #pragma unroll 1
         for (int j = 0; j < blocks && ok; ++j, ++n) {
-          const bool last = j + 1 == blocks;
-          if (last) {
-            item_done(k);
-            ++k;
-            more = fetch(next_tiles, next_blocks);
-          }
+          const int s = n & 1;
+          const uint32_t ph = (n >> 1) & 1;
 #pragma unroll 1
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (t < tiles) ok = values(t, n, j == 0, t == tiles - 1);
-            const int nt = last ? (more ? next_tiles : 0) : tiles;
-            if (ok && t < nt) ok = scores(t, n + 1, last, last ? next_blocks == 1 : j + 2 == blocks, t == nt - 1);
+          for (int t = 0; t < tiles && ok; ++t) {
+            if (!is_v) {
+              if (j == 0) {
+                ok = attn_wait(bars.q_full + 8 * t, (items >> t) & 1, abort, p.err);
+                items ^= 1u << t;
+              }
+              if (t == 0) ok = ok && attn_wait(bars.k_full + 8 * s, ph, abort, p.err);
+              // the tiles share S: the last scores have been read
+              if (made) ok = ok && attn_wait(bars.s_free, (made - 1) & 1, abort, p.err);
+              if (!ok) break;
+              ++made;
+              pr_fence_after();
+              if (pr_elect()) {
+                const uint32_t da = pr_desc(q_at + t * L::tile, 16), db = pr_desc(k_at + s * L::tile, 16);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                  const uint32_t off = ((i >> 2) * kBlock + (i & 3) * 32) >> 4;
+                  pr_mma_ss(tm + L::s_col, da + off, db + off, id_s, i > 0);
+                }
+                pr_commit(bars.s_full + 8 * t);
+                if (t == tiles - 1) pr_commit(bars.k_empty + 8 * s);
+                if (j == blocks - 1) pr_commit(bars.q_empty + 8 * t);
+              }
+            } else {
+              if (j == 0) {
+                // the tile's previous results have been read
+                if ((any >> t) & 1) ok = attn_wait(bars.o_empty + 8 * t, ((items >> t) & 1) ^ 1, abort, p.err);
+                any |= 1u << t;
+                items ^= 1u << t;
+              }
+              if (t == 0) ok = ok && attn_wait(bars.v_full + 8 * s, ph, abort, p.err);
+              ok = ok && attn_wait(bars.p_full + 8 * t, (valued >> t) & 1, abort, p.err);
+              if (!ok) break;
+              valued ^= 1u << t;
+              pr_fence_after();
+              if (pr_elect()) {
+                const uint32_t d = tm + L::o_col + t * D, at = tm + L::p_col + t * (kPrRows / 2);
+                const uint32_t db = pr_desc(v_at + s * L::tile, kBlock);
+#pragma unroll
+                for (int i = 0; i < kPrRows / 16; ++i) pr_mma_ts(d, at + 8 * i, db + i * (2048 >> 4), id_o, j > 0 || i > 0);
+                pr_commit(bars.o_done + 8 * t);
+                if (t == tiles - 1) pr_commit(bars.v_empty + 8 * s);
+              }
+            }
+            __syncwarp();
           }
         }
-        have = more;
-        tiles = next_tiles;
-        blocks = next_blocks;
       }
-      if (pr_elect()) pr_commit(bars.drain);              // whatever was issued has ended before the memory is given back
-      mbar_wait_bounded_warp(bars.drain, 0);
+      if (pr_elect()) pr_commit(bars.drain + 8 * is_v);   // whatever was issued has ended before the memory is given back
+      mbar_wait_bounded_warp(bars.drain + 8 * is_v, 0);
     }
   }
   __syncwarp();
   pr_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     pr_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPrTmemCols));
   }
