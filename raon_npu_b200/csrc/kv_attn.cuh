@@ -46,10 +46,10 @@ __device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N]) {
   }
 }
 
-// A warp's wait for a phase of an mbarrier: one verdict for all lanes, false
-// when it gave up (about a second of clock cycles) or another warp had
-// (``abort``), so that every role runs to its end.
-__device__ __forceinline__ bool attn_wait(uint32_t bar, uint32_t parity, volatile int *abort, int *err) {
+// A wait for a phase of an mbarrier that gives up after about a second of
+// clock cycles, or when another warp has (``abort``), so that every role runs
+// to its end: by one thread, and by a warp with one verdict for all lanes.
+__device__ __forceinline__ bool attn_wait1(uint32_t bar, uint32_t parity, volatile int *abort, int *err) {
   bool there = mbar_try_wait(bar, parity);
   if (!there) {
     const uint32_t t0 = (uint32_t)clock();
@@ -61,7 +61,10 @@ __device__ __forceinline__ bool attn_wait(uint32_t bar, uint32_t parity, volatil
       if (*abort) break;
     }
   }
-  return __all_sync(0xffffffffu, there);
+  return there;
+}
+__device__ __forceinline__ bool attn_wait(uint32_t bar, uint32_t parity, volatile int *abort, int *err) {
+  return __all_sync(0xffffffffu, attn_wait1(bar, parity, abort, err));
 }
 
 struct AttnParams {

@@ -397,6 +397,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           uint32_t v[4][32];
 #pragma unroll
           for (int i = 0; i < 4; ++i) pr_ld32(s_at + 32 * i, v[i]);
+          pr_wait_ld(v[0]);
+          pr_touch(v[1]);
+          pr_touch(v[2]);
+          pr_touch(v[3]);
+          pr_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars.s_free);
           if (j == 0) {
             c_row = crow[(k & 1) * 2 * kPrRows + t * kPrRows + row];
             if (c_row != c_row) c_row = 0.f, nan_groups = (1u << NJ) - 1u;
@@ -406,13 +413,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           const int4 f = info[(n + j) % kPrInfo];
           const float c = fmaxf(c_row * pow2f(-f.x), 0x1p-126f);   // above 0: a hidden score is -Inf
           const int c_hi = pos - t0, c_lo = p.window > 0 ? c_hi - p.window : INT_MIN, c_sink = p.sinks - t0;
-          pr_wait_ld(v[0]);
-          pr_touch(v[1]);
-          pr_touch(v[2]);
-          pr_touch(v[3]);
-          pr_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bars.s_free);
           if (masked) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -732,13 +732,14 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
       uint32_t items = 0, any = 0, made = 0, valued = 0;  // by tile (bit t): parity of its items, whether there were any ...
       int n = 0;                                          // ... of its values; scores of both tiles; blocks
       bool ok = true;
+      // the whole warp takes every step and one thread is elected for the products: their operands stay in uniform registers
 #pragma unroll 1
       for (int k = 0; ok; item_done(k), ++k) {
         ok = attn_wait(bars.item_full + 8 * (k & 1), (k >> 1) & 1, abort, p.err);
         if (!ok) break;
         const PrItem *it = reinterpret_cast<const PrItem *>(sm + L::o_item + 64 * (k & 1));
         if (it->b < 0) break;
-        const int tiles = it->tiles, blocks = it->blocks;
+        const int tiles = __shfl_sync(0xffffffffu, it->tiles, 0), blocks = __shfl_sync(0xffffffffu, it->blocks, 0);
 #pragma unroll 1
         for (int j = 0; j < blocks && ok; ++j, ++n) {
           const int s = n & 1;
