@@ -62,6 +62,7 @@ struct DcSeq {
   int first, rows, rows_do, len;   // first row, rows, rows computed (at most max_q), tokens
   int lo, sinks;                   // visible to some row: t >= lo or t < sinks
   int n_sink, stages, per_chunk, n_chunks;
+  __device__ int cost() const { return stages + n_chunks; }   // of one column block, in stages: an item costs one more
 };
 
 __device__ __forceinline__ DcSeq dc_seq(const AttnParams &p, int b) {
@@ -89,29 +90,63 @@ __device__ __forceinline__ int dc_stage(const DcItem &it, int v) {   // first to
 }
 __device__ __forceinline__ bool dc_seen(const DcItem &it, int t) { return t < it.len && (t >= it.lo || t < it.sinks); }
 
-__device__ __forceinline__ DcItem dc_item(const AttnParams &p, const int *prefix, int nc, int i) {
-  int lo = 0, hi = p.b.n_seqs - 1;   // the last sequence whose first item is <= i
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (prefix[mid] <= i) lo = mid;
-    else hi = mid - 1;
+// The items in order: sequences, kv heads, column blocks, chunks.  ``at`` is the cost of all items before the present one.
+struct DcWalk {
+  DcSeq s;
+  int b, cell, cells, chunk, at;
+
+  __device__ __forceinline__ void load(const AttnParams &p, int nc, int seq) {
+    b = seq;
+    s = dc_seq(p, seq);
+    cells = (s.rows_do * p.group + nc - 1) / nc * p.g.heads;
   }
-  const DcSeq s = dc_seq(p, lo);
-  DcItem it;
-  it.b = lo;
-  const int cbs = (s.rows_do * p.group + nc - 1) / nc;
-  int r = i - prefix[lo];
-  it.chunk = r % s.n_chunks;
-  r /= s.n_chunks;
-  it.cb = r % cbs;
-  it.head = r / cbs;
-  it.n_chunks = s.n_chunks;
-  it.first = s.first, it.rows = s.rows, it.rows_do = s.rows_do, it.len = s.len;
-  it.lo = s.lo, it.sinks = s.sinks, it.n_sink = s.n_sink;
-  it.v0 = it.chunk * s.per_chunk;
-  it.v1 = min(s.stages, it.v0 + s.per_chunk);
-  return it;
-}
+  // To the first item with at least ``cost`` before it.
+  __device__ __forceinline__ void seek(const AttnParams &p, const int *prefix, int nc, int cost) {
+    int lo = 0, hi = p.b.n_seqs - 1;   // the last sequence that starts at or before
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (prefix[mid] <= cost) lo = mid;
+      else hi = mid - 1;
+    }
+    load(p, nc, lo);
+    const int off = cost - prefix[lo];
+    cell = off / s.cost();
+    chunk = (off - cell * s.cost() + s.per_chunk) / (s.per_chunk + 1);
+    at = prefix[lo] + cell * s.cost() + chunk * (s.per_chunk + 1);
+    settle(p, nc);
+  }
+  // Past the end of a column block, of a sequence (which may have no rows).
+  __device__ __forceinline__ void settle(const AttnParams &p, int nc) {
+    if (cell < cells && chunk >= s.n_chunks) {
+      at += s.cost() - chunk * (s.per_chunk + 1);
+      chunk = 0;
+      ++cell;
+    }
+    while (cell >= cells && b + 1 < p.b.n_seqs) {
+      load(p, nc, b + 1);
+      cell = 0;
+    }
+  }
+  __device__ __forceinline__ void next(const AttnParams &p, int nc) {
+    ++chunk;
+    at += s.per_chunk + 1;
+    settle(p, nc);
+  }
+  __device__ __forceinline__ DcItem item(const AttnParams &p) const {
+    DcItem it;
+    it.b = b;
+    const int cbs = cells / p.g.heads;
+    it.head = cell / cbs;
+    it.cb = cell - it.head * cbs;
+    it.chunk = chunk;
+    it.n_chunks = s.n_chunks;
+    it.first = s.first, it.rows = s.rows, it.rows_do = s.rows_do, it.len = s.len;
+    it.lo = s.lo, it.sinks = s.sinks, it.n_sink = s.n_sink;
+    it.v0 = chunk * s.per_chunk;
+    it.v1 = min(s.stages, it.v0 + s.per_chunk);
+    return it;
+  }
+};
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   uint32_t d;
@@ -214,11 +249,11 @@ __global__ void __launch_bounds__(kDcThreads, 2) rc_kv_decode_kernel(const __gri
   }
   pdl_launch_dependents();
   pdl_wait_prior();
-  // items of every sequence, then their prefix sums
+  // cost of every sequence's items, then their prefix sums
 #pragma unroll 1
   for (int b = tid; b < a.b.n_seqs; b += kDcThreads) {
     const DcSeq s = dc_seq(a, b);
-    prefix[b + 1] = s.n_chunks * a.g.heads * ((s.rows_do * a.group + NC - 1) / NC);
+    prefix[b + 1] = s.cost() * a.g.heads * ((s.rows_do * a.group + NC - 1) / NC);
   }
   __syncthreads();
   if (warp == 0) {
@@ -242,16 +277,18 @@ __global__ void __launch_bounds__(kDcThreads, 2) rc_kv_decode_kernel(const __gri
 
   if (warp == kDcWarps) {
     // ----------------------------------------------------- items, copies --
-    const int items = prefix[a.b.n_seqs];
-    const int i0 = (int)((long long)blockIdx.x * items / gridDim.x), i1 = (int)((long long)(blockIdx.x + 1) * items / gridDim.x);
+    // this CTA's items: those that start in its share of the whole cost
+    const long long total = prefix[a.b.n_seqs];
+    const int end = (int)(total * (blockIdx.x + 1) / gridDim.x);
     const uint64_t policy = policy_evict_first();         // unless other column blocks come for the same tokens
     bool ok = true;
+    DcWalk w;
+    w.seek(a, prefix, NC, (int)(total * blockIdx.x / gridDim.x));
 #pragma unroll 1
-    for (int i = i0; i <= i1 && ok; ++i) {
-      const int k = i - i0;
+    for (int k = 0; ok; ++k, w.next(a, NC)) {
       DcItem it;
       it.b = -1;
-      if (i < i1) it = dc_item(a, prefix, NC, i);
+      if (w.cell < w.cells && w.at < end) it = w.item(a);
       ok = attn_wait(bar_taken + 8 * (k & 1), ((k >> 1) & 1) ^ 1, abort, a.err);
       if (!ok) break;
       if (lane == 0) {
@@ -738,7 +775,7 @@ static int decode_launch(rc_ctx *ctx, DcParams &p, int max_q, cudaStream_t s) {
   p.cbs = (int)(((long long)max_q * a.group + L::cols - 1) / L::cols);
   p.slots = (int)(chunks < kDcMaxChunks ? chunks : kDcMaxChunks) + kDcGroups;
   const long long cells = (long long)a.b.n_seqs * a.g.heads * p.cbs;
-  RC_CHECK_ARG(cells * p.slots <= INT_MAX, "rc_kv_attend: the batch is too large");
+  RC_CHECK_ARG(cells * (stages + kDcMaxChunks) <= INT_MAX, "rc_kv_attend: the batch is too large");
   int rc = ensure_attn_scratch(ctx, (size_t)cells * p.slots * L::cols * (L::D + 2) * sizeof(float), (size_t)cells * (kDcGroups + 1));
   if (rc) return rc;
   p.part = static_cast<float *>(ctx->attn_part);
