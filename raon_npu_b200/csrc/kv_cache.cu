@@ -7,13 +7,18 @@
 namespace rc {
 
 // ----------------------------------------------------------------- append --
-// One warp per (row, head); a lane holds E = D / 32 consecutive values.
-// Bound by memory latency and bandwidth: about 10 operations a value.  Query
-// heads are computed in 32 bits and rounded once to bf16.  Key and value heads
-// are computed and quantised in 64 bits: a code that falls on the other side
-// of a rounding boundary is off by a whole step, and the FP64 work (a few
-// operations for one value in q_heads/kv_heads + 2) hides under the loads.
+// A warp takes some heads of one row (``per_warp``: one when there are few
+// rows, up to eight when there are many, so that the row's position, its rotation
+// and the norm weights are fetched once for all of them); a lane holds E = D / 32
+// consecutive values, the next head's come in while this one is computed.
+// Bound by memory: about 10 operations a value.  Query heads are computed in 32
+// bits and rounded once to bf16.  Key heads are computed and quantised in 64
+// bits (a code on the other side of a rounding boundary is off by a whole step);
+// the FP64 work of one head in q_heads / kv_heads + 2 hides under the loads.
+// Value heads are taken as they come, so their codes are found in 32 bits and
+// only those near a boundary in 64.
 constexpr int kKvWarps = 8;
+constexpr int kAppendMaxHeads = 8;
 
 struct AppendParams {
   KvGeom g;
@@ -26,6 +31,7 @@ struct AppendParams {
   int rope_rows, rope_dim, interleaved;
   uint16_t *q_out;
   int ldq;
+  int per_warp, parts;   // heads of a warp, warps of a row
   int *err;
 };
 
@@ -55,13 +61,29 @@ __device__ __forceinline__ void load_lane(const void *x, size_t at, float (&v)[E
 __device__ __forceinline__ float inv_sqrt(float v) { return 1.f / sqrtf(v); }
 __device__ __forceinline__ double inv_sqrt(double v) { return 1.0 / sqrt(v); }
 
-// RMS norm of a head with weight w (null: none), then the rotation of its
-// first rd values by the table row (null: none).
+// A lane's part of the rotation of a row: cos and sin of its values' pairs.
+template <int E>
+struct RopeLane {
+  float c[E], s[E];   // of value e; interleaved pairs use the even entries
+  int half;           // rope_dim / 2; 0: no rotation
+
+  __device__ __forceinline__ void load(const float *row, int rd, bool interleaved, int lane) {
+    half = rd / 2;
+    const int d0 = lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = interleaved ? (d0 + e) / 2 : d0 + e < half ? d0 + e : d0 + e - half;
+      c[e] = d0 < rd ? row[i] : 1.f;
+      s[e] = d0 < rd ? row[half + i] : 0.f;
+    }
+  }
+};
+
+// RMS norm of a head with the lane's weights w (norm: whether there are any), then the rotation of its first values.
 template <int E, typename T>
-__device__ __forceinline__ void norm_rope(T (&v)[E], const uint16_t *w, float eps, const float *row, int rd,
+__device__ __forceinline__ void norm_rope(T (&v)[E], bool norm, const float (&w)[E], float eps, const RopeLane<E> &rope,
                                           bool interleaved, int lane) {
-  const int d0 = lane * E;
-  if (w) {
+  if (norm) {
     T ss = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) ss += v[e] * v[e];
@@ -69,72 +91,77 @@ __device__ __forceinline__ void norm_rope(T (&v)[E], const uint16_t *w, float ep
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const T r = inv_sqrt(ss / (T)(32 * E) + (T)eps);
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = v[e] * r * (T)bf16_to_f32(w[d0 + e]);
+    for (int e = 0; e < E; ++e) v[e] = v[e] * r * (T)w[e];
   }
-  if (!row) return;
-  const int half = rd / 2;
+  if (!rope.half) return;
   if (interleaved) {
-    if (d0 < rd) {
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const T c = row[(d0 + e) / 2], s = row[half + (d0 + e) / 2];
-        const T a = v[e], b = v[e + 1];
-        v[e] = a * c - b * s;
-        v[e + 1] = a * s + b * c;
-      }
+    for (int e = 0; e < E; e += 2) {
+      const T c = rope.c[e], s = rope.s[e], a = v[e], b = v[e + 1];
+      v[e] = a * c - b * s;
+      v[e + 1] = a * s + b * c;
     }
   } else {
-    const int off = half / E;   // lanes between the two values of a pair (rd is a multiple of 8)
-    const bool first = lane < off;
-    const int partner = first ? lane + off : (lane < 2 * off ? lane - off : lane);
+    const int off = rope.half / E;   // lanes between the two values of a pair (rope_dim is a multiple of 8)
+    const bool first = lane < off, second = !first && lane < 2 * off;
+    const int partner = first ? lane + off : second ? lane - off : lane;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const T other = __shfl_sync(0xffffffffu, v[e], partner);
-      if (d0 < rd) {
-        const int i = (first ? d0 : d0 - half) + e;
-        const T c = row[i], s = row[half + i];
-        v[e] = first ? v[e] * c - other * s : v[e] * c + other * s;
-      }
+      const T other = __shfl_sync(0xffffffffu, v[e], partner), c = rope.c[e], s = rope.s[e];
+      if (first) v[e] = v[e] * c - other * s;
+      if (second) v[e] = v[e] * c + other * s;
     }
   }
 }
 
-// The q4nx group rule in 64 bits over the 32 / E lanes of a group: codes of the
-// lane's values and the group's {scale, min}; a group without a finite form
-// becomes {0, NaN}.  Returns false for such a group.
-template <int E>
-__device__ __forceinline__ bool quantise_group(const double (&v)[E], uint32_t (&code)[E], uint32_t &param) {
+// The q4nx group rule in 64 bits: {scale, min} of a group from its extremes.  False when it has no finite form.
+__device__ __forceinline__ bool group_scale(double lo, double hi, float &sc, float &mn) {
+  mn = bf16_floor_f32(__double2float_rd(lo));
+  const double base = (double)mn, span = hi - base;
+  sc = bf16_ceil_f64(span / 15.0);
+  if (isfinite(sc) && base + 15.0 * (double)sc < hi) sc = bf16_next_up(sc);   // one step covers the rounding of the quotient
+  if (span == 0.0) sc = 0.f;
+  return isfinite(sc) && isfinite(mn);
+}
+__device__ __forceinline__ uint32_t group_code(double v, double base, float sc) {
+  const double q = sc > 0.f ? rint((v - base) / (double)sc) : 0.0;
+  return (uint32_t)(q < 0.0 ? 0.0 : q > 15.0 ? 15.0 : q);
+}
+
+// Codes of a lane's values and the group's {scale, min}, over the 32 / E lanes of a group; a group without a finite
+// form becomes {0, NaN} (and false is returned).  T = float: the codes in 32 bits, which are those of 64 unless the
+// quotient lies within 1e-3 of a boundary or the numbers are extreme.
+template <int E, typename T>
+__device__ __forceinline__ bool quantise_group(const T (&v)[E], uint32_t (&code)[E], uint32_t &param) {
   constexpr int kLanes = kKvGroup / E;
   bool fine = true;
-  double lo = v[0], hi = v[0];
+  T lo = v[0], hi = v[0];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     fine = fine && isfinite(v[e]);
-    lo = fmin(lo, v[e]);
-    hi = fmax(hi, v[e]);
+    lo = v[e] < lo ? v[e] : lo;
+    hi = v[e] > hi ? v[e] : hi;
   }
 #pragma unroll
   for (int o = 1; o < kLanes; o <<= 1) {
-    lo = fmin(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmax(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    const T a = __shfl_xor_sync(0xffffffffu, lo, o), b = __shfl_xor_sync(0xffffffffu, hi, o);
+    lo = a < lo ? a : lo;
+    hi = b > hi ? b : hi;
   }
   const int lane = threadIdx.x & 31;
-  const unsigned mine = ((kLanes == 32 ? 0u : (1u << (kLanes & 31))) - 1u) << (lane & ~(kLanes - 1));
+  const unsigned mine = ((1u << kLanes) - 1u) << (lane & ~(kLanes - 1));
   fine = (__ballot_sync(0xffffffffu, fine) & mine) == mine;
-  const float mn = bf16_floor_f32(__double2float_rd(lo));
-  const double base = (double)mn, span = hi - base;
-  float sc = bf16_ceil_f64(span / 15.0);
-  if (fine && isfinite(sc) && base + 15.0 * (double)sc < hi) sc = bf16_next_up(sc);   // one step covers the rounding of the quotient
-  if (span == 0.0) sc = 0.f;
-  fine = fine && isfinite(sc) && isfinite(mn);
-  const double inv = sc > 0.f ? 1.0 / (double)sc : 0.0;
+  float sc, mn;
+  fine = group_scale((double)lo, (double)hi, sc, mn) && fine;
+  const T inv = sc > 0.f ? (T)1 / (T)sc : (T)0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const double t = (v[e] - base) * inv;
-    double q = rint(t);
-    if (fabs(fabs(t - q) - 0.5) < 1e-6 && sc > 0.f) q = rint((v[e] - base) / (double)sc);   // ties: the exact quotient
-    q = q < 0.0 ? 0.0 : (q > 15.0 ? 15.0 : q);
-    code[e] = fine ? (uint32_t)q : 0u;
+    const T d = v[e] - (T)mn, t = d * inv, q = rint(t);
+    const T near = sizeof(T) == 4 ? (T)1e-3 : (T)1e-6;   // of a boundary: the exact quotient decides
+    const bool sure = fabs(fabs(t - q) - (T)0.5) > near && (sizeof(T) == 8 || (fabs(d) < (T)1e38 && sc > 1e-30f));
+    code[e] = sure ? (uint32_t)(q < (T)0 ? (T)0 : q > (T)15 ? (T)15 : q) : 0u;
+    if (!sure) code[e] = group_code((double)v[e], (double)mn, sc);
+    if (!fine) code[e] = 0u;
   }
   param = fine ? (__float_as_uint(sc) >> 16) | (__float_as_uint(mn) & 0xFFFF0000u) : 0x7FC00000u;
   return fine;
@@ -145,58 +172,79 @@ __global__ void __launch_bounds__(32 * kKvWarps) rc_kv_append_kernel(const __gri
   constexpr int D = 32 * E, NJ = D / kKvGroup;
   pdl_launch_dependents();
   pdl_wait_prior();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, d0 = lane * E;
   const int n_heads = p.q_heads + 2 * p.g.heads;
   const long long item = (long long)blockIdx.x * kKvWarps + (threadIdx.x >> 5);
-  const int r = (int)(item / n_heads), h = (int)(item % n_heads);
+  const int r = (int)(item / p.parts), h0 = (int)(item - (long long)r * p.parts) * p.per_warp;
+  const int h1 = min(h0 + p.per_warp, n_heads);
   if (r >= p.b.n_rows) return;
-  float x[E];
-  load_lane<E, F32>(p.x, (size_t)r * p.ldx + h * D + lane * E, x);
+  const size_t x_at = (size_t)r * p.ldx + d0;
+  float next[E];
+  load_lane<E, F32>(p.x, x_at + (size_t)h0 * D, next);
+  float wq[E], wk[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    wq[e] = p.q_norm && h0 < p.q_heads ? bf16_to_f32(p.q_norm[d0 + e]) : 1.f;
+    wk[e] = p.k_norm && h1 > p.q_heads ? bf16_to_f32(p.k_norm[d0 + e]) : 1.f;
+  }
   int seq, pos;
   if (!kv_find_row(p.b, r, lane, seq, pos)) return;
-  const bool is_q = h < p.q_heads, is_v = h >= p.q_heads + p.g.heads;
-  const float *row = nullptr;
-  if (p.rope && !is_v && pos >= 0) {
+  RopeLane<E> rope;
+  rope.half = 0;
+  if (p.rope && pos >= 0 && h0 < p.q_heads + p.g.heads) {
     if (pos >= p.rope_rows) {
       if (lane == 0) atomicCAS(p.err, 0, kErrKvRange);
       return;
     }
-    row = p.rope + (size_t)pos * p.rope_dim;
+    rope.load(p.rope + (size_t)pos * p.rope_dim, p.rope_dim, p.interleaved, lane);
   }
-  if (is_q) {
-    norm_rope<E, float>(x, p.q_norm, p.eps, row, p.rope_dim, p.interleaved, lane);
-    uint16_t *out = p.q_out + (size_t)r * p.ldq + h * D + lane * E;
-    uint32_t w[E / 2];
+  uint8_t *page = h1 > p.q_heads && pos >= 0 ? kv_head_block(p.g, p.b, seq, pos, 0, p.err) : nullptr;
+  const int t = pos & (p.g.page - 1);
+#pragma unroll 1
+  for (int h = h0; h < h1; ++h) {
+    float x[E];
 #pragma unroll
-    for (int e = 0; e < E; e += 2)
-      w[e / 2] = f32_to_bf16_rne(x[e]) | ((uint32_t)f32_to_bf16_rne(x[e + 1]) << 16);
-    if constexpr (E == 4) *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t *>(out) = w[0];
-    return;
+    for (int e = 0; e < E; ++e) x[e] = next[e];
+    if (h + 1 < h1) load_lane<E, F32>(p.x, x_at + (size_t)(h + 1) * D, next);
+    if (h < p.q_heads) {
+      norm_rope<E, float>(x, p.q_norm != nullptr, wq, p.eps, rope, p.interleaved, lane);
+      uint16_t *out = p.q_out + (size_t)r * p.ldq + h * D + d0;
+      uint32_t w[E / 2];
+#pragma unroll
+      for (int e = 0; e < E; e += 2)
+        w[e / 2] = f32_to_bf16_rne(x[e]) | ((uint32_t)f32_to_bf16_rne(x[e + 1]) << 16);
+      if constexpr (E == 4) *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t *>(out) = w[0];
+      continue;
+    }
+    if (!page) return;
+    const bool is_v = h >= p.q_heads + p.g.heads;
+    uint32_t code[E], param;
+    bool fine;
+    if (is_v) {
+      fine = quantise_group<E, float>(x, code, param);
+    } else {
+      double k[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) k[e] = x[e];
+      norm_rope<E, double>(k, p.k_norm != nullptr, wk, p.eps, rope, p.interleaved, lane);
+      fine = quantise_group<E, double>(k, code, param);
+    }
+    if (!fine) atomicCAS(p.err, 0, kErrKvNonFinite);
+    uint8_t *blk = page + (size_t)(h - p.q_heads - (is_v ? p.g.heads : 0)) * p.g.head_bytes;
+    uint8_t *codes = blk + (is_v ? p.g.vc_off : 0) + t * (D / 2) + (is_v ? kv_v_byte(d0, NJ) : kv_k_byte(d0, NJ));
+    if constexpr (E == 4)
+      *reinterpret_cast<uint16_t *>(codes) = (uint16_t)(code[0] | (code[1] << 4) | (code[2] << 8) | (code[3] << 12));
+    else
+      *codes = (uint8_t)(code[0] | (code[1] << 4));
+    if (d0 % kKvGroup == 0)
+      reinterpret_cast<uint32_t *>(blk + (is_v ? p.g.vp_off : p.g.kp_off))[t * NJ + d0 / kKvGroup] = param;
   }
-  if (pos < 0) return;
-  const int head = is_v ? h - p.q_heads - p.g.heads : h - p.q_heads;
-  uint8_t *blk = kv_head_block(p.g, p.b, seq, pos, head, p.err);
-  if (!blk) return;
-  double v[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = x[e];
-  if (!is_v) norm_rope<E, double>(v, p.k_norm, p.eps, row, p.rope_dim, p.interleaved, lane);
-  uint32_t code[E], param;
-  if (!quantise_group<E>(v, code, param)) atomicCAS(p.err, 0, kErrKvNonFinite);
-  const int t = pos & (p.g.page - 1), d0 = lane * E;
-  uint8_t *codes = blk + (is_v ? p.g.vc_off : 0) + (size_t)t * (D / 2) + (is_v ? kv_v_byte(d0, NJ) : kv_k_byte(d0, NJ));
-  if constexpr (E == 4)
-    *reinterpret_cast<uint16_t *>(codes) = (uint16_t)(code[0] | (code[1] << 4) | (code[2] << 8) | (code[3] << 12));
-  else
-    *codes = (uint8_t)(code[0] | (code[1] << 4));
-  if (d0 % kKvGroup == 0)
-    reinterpret_cast<uint32_t *>(blk + (is_v ? p.g.vp_off : p.g.kp_off))[t * NJ + d0 / kKvGroup] = param;
 }
 
 // ------------------------------------------------------------------- read --
-// One warp per (row, kv head): both rows of the head, min + scale * code in
-// 32 bits (one rounding: scale * code is exact), rounded to bf16.
+// One warp per (row, kv head, K or V): min + scale * code in 32 bits (one
+// rounding: scale * code is exact), rounded to bf16.
 template <int E>
 __global__ void __launch_bounds__(32 * kKvWarps)
     rc_kv_read_kernel(const __grid_constant__ KvGeom g, const __grid_constant__ KvBatchDev b, uint16_t *k_out,
@@ -206,32 +254,32 @@ __global__ void __launch_bounds__(32 * kKvWarps)
   pdl_wait_prior();
   const int lane = threadIdx.x & 31, d0 = lane * E;
   const long long item = (long long)blockIdx.x * kKvWarps + (threadIdx.x >> 5);
-  const int r = (int)(item / g.heads), h = (int)(item % g.heads);
+  const int r = (int)(item / (2 * g.heads)), i = (int)(item - (long long)r * 2 * g.heads);
+  const int kv = i >= g.heads ? 1 : 0, h = i - kv * g.heads;
   if (r >= b.n_rows) return;
   int seq, pos;
   if (!kv_find_row(b, r, lane, seq, pos)) return;
   const uint8_t *blk = pos >= 0 ? kv_head_block(g, b, seq, pos, h, err) : nullptr;
   const int t = pos & (g.page - 1);
+  uint32_t w[E / 2];
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    uint32_t w[E / 2];
+  for (int e = 0; e < E / 2; ++e) w[e] = 0;
+  if (blk) {
+    const uint8_t *codes = blk + (kv ? g.vc_off : 0) + t * (D / 2) + (kv ? kv_v_byte(d0, NJ) : kv_k_byte(d0, NJ));
+    const uint32_t par = __ldcg(reinterpret_cast<const uint32_t *>(blk + (kv ? g.vp_off : g.kp_off)) + t * NJ + d0 / kKvGroup);
+    uint32_t nib;
+    if constexpr (E == 4) nib = __ldcg(reinterpret_cast<const uint16_t *>(codes));
+    else nib = __ldcg(codes);
+    const float sc = bf16_lo_f32(par), mn = bf16_hi_f32(par);
 #pragma unroll
-    for (int i = 0; i < E / 2; ++i) w[i] = 0;
-    if (blk) {
-      const uint8_t *codes = blk + (kv ? g.vc_off : 0) + (size_t)t * (D / 2) + (kv ? kv_v_byte(d0, NJ) : kv_k_byte(d0, NJ));
-      const uint32_t par = __ldcg(reinterpret_cast<const uint32_t *>(blk + (kv ? g.vp_off : g.kp_off)) + t * NJ + d0 / kKvGroup);
-      const float sc = bf16_lo_f32(par), mn = bf16_hi_f32(par);
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        const uint32_t byte = __ldcg(codes + i);
-        const float a = fmaf(sc, (float)(byte & 15), mn), c = fmaf(sc, (float)(byte >> 4), mn);
-        w[i] = f32_to_bf16_rne(a) | ((uint32_t)f32_to_bf16_rne(c) << 16);
-      }
+    for (int e = 0; e < E / 2; ++e) {
+      const float a = fmaf(sc, (float)(nib >> (8 * e) & 15), mn), c = fmaf(sc, (float)(nib >> (8 * e + 4) & 15), mn);
+      w[e] = f32_to_bf16_rne(a) | ((uint32_t)f32_to_bf16_rne(c) << 16);
     }
-    uint16_t *out = (kv ? v_out : k_out) + ((size_t)r * g.heads + h) * D + d0;
-    if constexpr (E == 4) *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t *>(out) = w[0];
   }
+  uint16_t *out = (kv ? v_out : k_out) + ((size_t)r * g.heads + h) * D + d0;
+  if constexpr (E == 4) *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t *>(out) = w[0];
 }
 
 // ------------------------------------------------------------- page moves --
@@ -454,8 +502,12 @@ int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, 
   p.q_out = q_out_dev;
   p.ldq = ldq;
   p.err = kv->ctx->err;
-  const long long items = (long long)n_rows * (q_heads + 2 * kv->heads);
-  const long long blocks = (items + kKvWarps - 1) / kKvWarps;
+  // as many heads a warp as leave 64 warps an SM
+  const int heads = q_heads + 2 * kv->heads;
+  const long long spare = (long long)n_rows * heads / (64ll * kv->ctx->sm_count);
+  p.per_warp = spare < 1 ? 1 : spare < kAppendMaxHeads ? (int)spare : kAppendMaxHeads;
+  p.parts = (heads + p.per_warp - 1) / p.per_warp;
+  const long long blocks = ((long long)n_rows * p.parts + kKvWarps - 1) / kKvWarps;
   RC_CHECK_ARG(blocks <= INT_MAX, "rc_kv_append: too many rows (%d)", n_rows);
   const dim3 grid((unsigned)blocks), block(32 * kKvWarps);
   const cudaStream_t s = pick_stream(kv->ctx, stream);
@@ -474,7 +526,7 @@ int rc_kv_read(rc_kv *kv, int layer, int n_rows, const int32_t *table_dev, int c
   RC_CUDA_TRY(cudaSetDevice(kv->ctx->device));
   const KvGeom g = kv_geom(kv, layer);
   const KvBatchDev b{table_dev, kv_len_dev, q_off_dev, cols, ld_table, n_seqs, n_rows};
-  const long long blocks = ((long long)n_rows * kv->heads + kKvWarps - 1) / kKvWarps;
+  const long long blocks = ((long long)n_rows * 2 * kv->heads + kKvWarps - 1) / kKvWarps;
   RC_CHECK_ARG(blocks <= INT_MAX, "rc_kv_read: too many rows (%d)", n_rows);
   const dim3 grid((unsigned)blocks), block(32 * kKvWarps);
   const cudaStream_t s = pick_stream(kv->ctx, stream);

@@ -42,10 +42,12 @@ namespace rc {
 constexpr int kDcWarps = 4;                       // computing warps
 constexpr int kDcThreads = 32 * (kDcWarps + 1);   // and one that copies
 constexpr int kDcStage = 128;                     // tokens of a stage
-// A chunk is an eighth of the stages, but two to eight of them (256 to 1024
-// tokens: fewer cost more in partial results than they give in parallel work),
-// and a 128th where that is more.
-constexpr int kDcMinStages = 2, kDcMaxStages = 8, kDcMaxChunks = 128;
+// A chunk is an eighth of the stages, but two to six of them (256 to 768
+// tokens: smaller ones cost more in partial results than they give in balance;
+// 64 sequences of up to 8191 tokens took 68.7 / 67.4 / 67.4 us with at most 4 /
+// 6 / 8, two of up to 131072 65.7 / 55.3 / 62.6 us), and a 256th where that is
+// more.
+constexpr int kDcMinStages = 2, kDcMaxStages = 6, kDcMaxChunks = 256;
 constexpr int kDcFan = 16;                        // partial results joined at a time
 constexpr int kDcGroups = (kDcMaxChunks + kDcFan - 1) / kDcFan;
 
@@ -159,7 +161,7 @@ template <int NJ, int NB>
 struct DcLayout {
   static constexpr int D = 32 * NJ, cols = 8 * NB;
   static constexpr int stage = kDcStage * D * 5 / 4;
-  static constexpr int stages = NJ == 4 ? (NB == 1 ? 4 : 3) : (NB == 1 ? 8 : 6);
+  static constexpr int stages = NJ == 4 ? (NB == 1 ? 2 : 3) : (NB == 1 ? 5 : 6);
   static constexpr int join = kDcWarps * cols * D * 4;                       // the warps' values of one item
   static_assert(join >= cols * kDcFan * 8, "the joined parts' (reference, sum) lie there too");
   static constexpr int o_scratch = stages * stage;
@@ -173,20 +175,19 @@ struct DcLayout {
   static int bytes(int n_seqs) { return o_prefix + (n_seqs + 1) * 4; }
 };
 
-// The CTA's writes are out; true in every thread of the CTA that arrives last
-// of n, which then sees the others' writes (and finds the counter at zero again).
+// True in every thread of the CTA that arrives last of n; it then sees what the
+// others wrote before they arrived (and leaves the counter at zero).  One thread's
+// releasing add after the barrier covers the CTA's writes.
 __device__ __forceinline__ bool dc_arrive_last(int *count, int n, volatile int *s_last, int tid) {
-  __threadfence();
   dc_sync();
   if (tid == 0) {
-    const bool last = atomicAdd(count, 1) == n - 1;
-    *s_last = last;
-    if (last) *count = 0;
+    int before;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+    *s_last = before == n - 1;
+    if (before == n - 1) *count = 0;
   }
   dc_sync();
-  if (!*s_last) return false;
-  __threadfence();
-  return true;
+  return *s_last;
 }
 
 // Joins n <= kDcFan partial results in order; sink(column, value, 4 sums, reference, sum).
@@ -223,7 +224,7 @@ __device__ __forceinline__ void dc_join(const float *src, int n, float *scratch,
 
 // MULTI: the rows of a sequence have masks of their own.
 template <int NJ, int NB, bool MULTI>
-__global__ void __launch_bounds__(kDcThreads, 2) rc_kv_decode_kernel(const __grid_constant__ DcParams p) {
+__global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kernel(const __grid_constant__ DcParams p) {
   using L = DcLayout<NJ, NB>;
   constexpr int D = L::D, NC = L::cols;
   extern __shared__ __align__(128) uint8_t sm[];
