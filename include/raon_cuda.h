@@ -411,7 +411,7 @@ int rc_kv_destroy(rc_kv *kv);
  * is given: rope [rope_rows][rope_dim] f32 holds cos | sin (rope_dim / 2 each)
  * of a position; the first rope_dim values of a head turn in pairs
  * (i, i + rope_dim/2), or (2i, 2i+1) when interleaved != 0; rope_dim is a
- * multiple of 8, at most head_dim.  Queries go to q_out [n_rows][ldq] bf16;
+ * multiple of 16, at most head_dim.  Queries go to q_out [n_rows][ldq] bf16;
  * keys and values are quantised (the group rule of rc_quantize_q4nx: bf16
  * floor of the minimum, bf16 ceiling of (max - min) / 15 stepped up until it
  * covers the maximum, nearest code, ties to even), in 64 bits throughout, and

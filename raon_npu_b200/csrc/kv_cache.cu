@@ -7,18 +7,21 @@
 namespace rc {
 
 // ----------------------------------------------------------------- append --
-// A warp takes some heads of one row (``per_warp``: one when there are few
-// rows, up to eight when there are many, so that the row's position, its rotation
-// and the norm weights are fetched once for all of them); a lane holds E = D / 32
-// consecutive values, the next head's come in while this one is computed.
-// Bound by memory: about 10 operations a value.  Query heads are computed in 32
-// bits and rounded once to bf16.  Key heads are computed and quantised in 64
-// bits (a code on the other side of a rounding boundary is off by a whole step);
-// the FP64 work of one head in q_heads / kv_heads + 2 hides under the loads.
-// Value heads are taken as they come, so their codes are found in 32 bits and
-// only those near a boundary in 64.
-constexpr int kKvWarps = 8;
-constexpr int kAppendMaxHeads = 8;
+// A lane holds 8 consecutive values, so a warp holds 256 / D heads (a unit).  A
+// warp takes units of one row: one when there are few rows, up to four, all
+// asked for at once, when there are many, so that the row's position, its
+// rotation and the norm weights are fetched once for all of them and enough
+// loads are in flight.  Bound by memory where there are many rows (about 10
+// operations a value, 5 instructions for 8 values to reduce a sum: with 4 values
+// a lane the shuffles and conversions took more time than the loads).  Query
+// heads are computed in 32 bits and rounded once to bf16.  Key heads are
+// normalised, rotated and scaled in 64 bits (a code on the other side of a
+// rounding boundary is off by a whole step), value heads are taken as they come;
+// the codes of both are found in 32 bits and those near a boundary once more in
+// 64.  A block is one warp, so that the room of a short one (queries) is free
+// before a long one (keys) ends: 4096 rows of 32 + 8 + 8 heads of 128 with their
+// read-back take 47 us, with blocks of two warps 50 and of eight 65.
+constexpr int kAppendUnits = 4, kAppendCtas = 24;
 
 struct AppendParams {
   KvGeom g;
@@ -31,255 +34,269 @@ struct AppendParams {
   int rope_rows, rope_dim, interleaved;
   uint16_t *q_out;
   int ldq;
-  int per_warp, parts;   // heads of a warp, warps of a row
+  int units, parts_q, parts;   // units of a warp; warps for the queries of a row, for the row
   int *err;
 };
 
-template <int E, bool F32>
-__device__ __forceinline__ void load_lane(const void *x, size_t at, float (&v)[E]) {
-  if constexpr (F32) {
-    const float *p = static_cast<const float *>(x) + at;
-    if constexpr (E == 4) {
-      const float4 w = __ldcg(reinterpret_cast<const float4 *>(p));
-      v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+template <bool F32>
+struct Raw8 {
+  uint4 a, b;   // 8 bf16 in a, or 8 f32
+  __device__ __forceinline__ void load(const void *x, size_t at) {
+    if constexpr (F32) {
+      a = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const float *>(x) + at));
+      b = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const float *>(x) + at) + 1);
     } else {
-      const float2 w = __ldcg(reinterpret_cast<const float2 *>(p));
-      v[0] = w.x, v[1] = w.y;
-    }
-  } else {
-    const uint16_t *p = static_cast<const uint16_t *>(x) + at;
-    if constexpr (E == 4) {
-      const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(p));
-      v[0] = bf16_lo_f32(w.x), v[1] = bf16_hi_f32(w.x), v[2] = bf16_lo_f32(w.y), v[3] = bf16_hi_f32(w.y);
-    } else {
-      const uint32_t w = __ldcg(reinterpret_cast<const uint32_t *>(p));
-      v[0] = bf16_lo_f32(w), v[1] = bf16_hi_f32(w);
+      a = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(x) + at));
     }
   }
-}
-
-__device__ __forceinline__ float inv_sqrt(float v) { return 1.f / sqrtf(v); }
-__device__ __forceinline__ double inv_sqrt(double v) { return 1.0 / sqrt(v); }
-
-// A lane's part of the rotation of a row: cos and sin of its values' pairs.
-template <int E>
-struct RopeLane {
-  float c[E], s[E];   // of value e; interleaved pairs use the even entries
-  int half;           // rope_dim / 2; 0: no rotation
-
-  __device__ __forceinline__ void load(const float *row, int rd, bool interleaved, int lane) {
-    half = rd / 2;
-    const int d0 = lane * E;
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    if constexpr (F32) {
+      const uint32_t u[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = interleaved ? (d0 + e) / 2 : d0 + e < half ? d0 + e : d0 + e - half;
-      c[e] = d0 < rd ? row[i] : 1.f;
-      s[e] = d0 < rd ? row[half + i] : 0.f;
+      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]), v[4 + i] = __uint_as_float(u[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo_f32(w[i]), v[2 * i + 1] = bf16_hi_f32(w[i]);
     }
   }
 };
 
-// RMS norm of a head with the lane's weights w (norm: whether there are any), then the rotation of its first values.
-template <int E, typename T>
-__device__ __forceinline__ void norm_rope(T (&v)[E], bool norm, const float (&w)[E], float eps, const RopeLane<E> &rope,
-                                          bool interleaved, int lane) {
-  if (norm) {
+__device__ __forceinline__ uint32_t bf16x2_rn(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ uint4 bf16x8_rn(const float (&v)[8]) {
+  return make_uint4(bf16x2_rn(v[0], v[1]), bf16x2_rn(v[2], v[3]), bf16x2_rn(v[4], v[5]), bf16x2_rn(v[6], v[7]));
+}
+
+__device__ __forceinline__ float inv_sqrt(float v) { return rsqrtf(v); }
+__device__ __forceinline__ double inv_sqrt(double v) { return rsqrt(v); }
+
+// A lane's part of the rotation of a row: v = c * v + s * (its pair's other value).
+struct RopeLane {
+  float c[8], s[8];
+  int partner;        // lane of the other values; this one when a pair lies within the lane (interleaved)
+  bool any;
+
+  __device__ __forceinline__ void load(const float *row, int rd, bool interleaved, int lane, int d0) {
+    const int half = rd / 2, off = half / 8;   // rope_dim is a multiple of 16
+    any = true;
+    partner = interleaved || d0 >= rd ? lane : d0 < half ? lane + off : lane - off;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = 1.f, s[e] = 0.f;
+    if (d0 >= rd) return;
+    if (interleaved) {
+      const float4 a = __ldcg(reinterpret_cast<const float4 *>(row + d0 / 2)),
+                   b = __ldcg(reinterpret_cast<const float4 *>(row + half + d0 / 2));
+      const float cs[4] = {a.x, a.y, a.z, a.w}, sn[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) c[e] = cs[e / 2], s[e] = e % 2 ? sn[e / 2] : -sn[e / 2];
+    } else {
+      const float4 *at = reinterpret_cast<const float4 *>(row + (d0 < half ? d0 : d0 - half));
+      const float4 a0 = __ldcg(at), a1 = __ldcg(at + 1), b0 = __ldcg(at + half / 4), b1 = __ldcg(at + half / 4 + 1);
+      const float cs[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+      const float sn[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) c[e] = cs[e], s[e] = d0 < half ? -sn[e] : sn[e];
+    }
+  }
+};
+
+// RMS norm of a head with the lane's weights w (norm: whether it has one), then the rotation (turn: whether it turns).
+template <int kLanes, typename T>
+__device__ __forceinline__ void norm_rope(T (&v)[8], bool norm, bool any_norm, const uint4 &w, float eps,
+                                          const RopeLane &rope, bool interleaved, bool turn) {
+  if (any_norm) {
     T ss = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) ss += v[e] * v[e];
+    for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const T r = inv_sqrt(ss / (T)(32 * E) + (T)eps);
+    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const T r = inv_sqrt(ss * (T)(1.0 / (8 * kLanes)) + (T)eps);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    if (norm)
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = v[e] * r * (T)w[e];
+      for (int e = 0; e < 8; ++e) v[e] = v[e] * r * (T)(e % 2 ? bf16_hi_f32(u[e / 2]) : bf16_lo_f32(u[e / 2]));
   }
-  if (!rope.half) return;
-  if (interleaved) {
+  if (!rope.any) return;
+  T other[8];
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const T c = rope.c[e], s = rope.s[e], a = v[e], b = v[e + 1];
-      v[e] = a * c - b * s;
-      v[e + 1] = a * s + b * c;
-    }
-  } else {
-    const int off = rope.half / E;   // lanes between the two values of a pair (rope_dim is a multiple of 8)
-    const bool first = lane < off, second = !first && lane < 2 * off;
-    const int partner = first ? lane + off : second ? lane - off : lane;
+  for (int e = 0; e < 8; ++e) other[e] = interleaved ? v[e ^ 1] : __shfl_sync(0xffffffffu, v[e], rope.partner);
+  if (turn)
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const T other = __shfl_sync(0xffffffffu, v[e], partner), c = rope.c[e], s = rope.s[e];
-      if (first) v[e] = v[e] * c - other * s;
-      if (second) v[e] = v[e] * c + other * s;
-    }
-  }
+    for (int e = 0; e < 8; ++e) v[e] = v[e] * (T)rope.c[e] + other[e] * (T)rope.s[e];
 }
 
 // The q4nx group rule in 64 bits: {scale, min} of a group from its extremes.  False when it has no finite form.
 __device__ __forceinline__ bool group_scale(double lo, double hi, float &sc, float &mn) {
   mn = bf16_floor_f32(__double2float_rd(lo));
   const double base = (double)mn, span = hi - base;
-  sc = bf16_ceil_f64(span / 15.0);
-  if (isfinite(sc) && base + 15.0 * (double)sc < hi) sc = bf16_next_up(sc);   // one step covers the rounding of the quotient
+  // The smallest bf16 that is at least span / 15: a candidate that may be one step low, then the exact comparison.
+  sc = bf16_ceil_f32(__double2float_rn(span) * (float)(0.999999 / 15.0));
+  if (15.0 * (double)sc < span) sc = bf16_next_up(sc);
+  if (base + 15.0 * (double)sc < hi) sc = bf16_next_up(sc);   // one step covers the rounding of the sum
   if (span == 0.0) sc = 0.f;
   return isfinite(sc) && isfinite(mn);
 }
-__device__ __forceinline__ uint32_t group_code(double v, double base, float sc) {
-  const double q = sc > 0.f ? rint((v - base) / (double)sc) : 0.0;
+__device__ __noinline__ uint32_t group_code(double v, float mn, float sc) {
+  const double q = sc > 0.f ? rint((v - (double)mn) / (double)sc) : 0.0;
   return (uint32_t)(q < 0.0 ? 0.0 : q > 15.0 ? 15.0 : q);
 }
 
-// Codes of a lane's values and the group's {scale, min}, over the 32 / E lanes of a group; a group without a finite
-// form becomes {0, NaN} (and false is returned).  T = float: the codes in 32 bits, which are those of 64 unless the
-// quotient lies within 1e-3 of a boundary or the numbers are extreme.
-template <int E, typename T>
-__device__ __forceinline__ bool quantise_group(const T (&v)[E], uint32_t (&code)[E], uint32_t &param) {
-  constexpr int kLanes = kKvGroup / E;
+// The lane's 8 codes (value e at bits 4e) and the group's {scale, min}, over the 4 lanes of a group; a group without a
+// finite form becomes {0, NaN} (and false is returned).  The quotient is good to 15 * 2^-22 in 32 bits: within 1e-5 of
+// a boundary, or where the numbers are extreme, the 64-bit one decides.
+template <typename T>
+__device__ __forceinline__ bool quantise_group(const T (&v)[8], uint32_t &codes, uint32_t &param) {
   bool fine = true;
   T lo = v[0], hi = v[0];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
+  for (int e = 0; e < 8; ++e) {
     fine = fine && isfinite(v[e]);
     lo = v[e] < lo ? v[e] : lo;
     hi = v[e] > hi ? v[e] : hi;
   }
 #pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) {
+  for (int o = 1; o < 4; o <<= 1) {
     const T a = __shfl_xor_sync(0xffffffffu, lo, o), b = __shfl_xor_sync(0xffffffffu, hi, o);
     lo = a < lo ? a : lo;
     hi = b > hi ? b : hi;
   }
-  const int lane = threadIdx.x & 31;
-  const unsigned mine = ((1u << kLanes) - 1u) << (lane & ~(kLanes - 1));
+  const unsigned mine = 0xFu << (threadIdx.x & 28);
   fine = (__ballot_sync(0xffffffffu, fine) & mine) == mine;
   float sc, mn;
   fine = group_scale((double)lo, (double)hi, sc, mn) && fine;
-  const T inv = sc > 0.f ? (T)1 / (T)sc : (T)0;
+  const float inv = sc > 0.f ? __frcp_rn(sc) : 0.f;
+  const bool plain = fabs(hi) < (T)1e37 && fabs(lo) < (T)1e37 && sc > 1e-30f;
+  codes = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const T d = v[e] - (T)mn, t = d * inv, q = rint(t);
-    const T near = sizeof(T) == 4 ? (T)1e-3 : (T)1e-6;   // of a boundary: the exact quotient decides
-    const bool sure = fabs(fabs(t - q) - (T)0.5) > near && (sizeof(T) == 8 || (fabs(d) < (T)1e38 && sc > 1e-30f));
-    code[e] = sure ? (uint32_t)(q < (T)0 ? (T)0 : q > (T)15 ? (T)15 : q) : 0u;
-    if (!sure) code[e] = group_code((double)v[e], (double)mn, sc);
-    if (!fine) code[e] = 0u;
+  for (int e = 0; e < 8; ++e) {
+    const float t = (float)(v[e] - (T)mn) * inv, q = rintf(t);
+    uint32_t c = (uint32_t)fminf(fmaxf(q, 0.f), 15.f);
+    if (!plain || fabsf(fabsf(t - q) - 0.5f) < 1e-5f) c = group_code((double)v[e], mn, sc);
+    codes |= c << (4 * e);
   }
+  if (!fine) codes = 0;
   param = fine ? (__float_as_uint(sc) >> 16) | (__float_as_uint(mn) & 0xFFFF0000u) : 0x7FC00000u;
   return fine;
 }
 
-template <int E, bool F32>
-__global__ void __launch_bounds__(32 * kKvWarps) rc_kv_append_kernel(const __grid_constant__ AppendParams p) {
-  constexpr int D = 32 * E, NJ = D / kKvGroup;
+template <int NJ, bool F32>
+__global__ void __launch_bounds__(32, kAppendCtas) rc_kv_append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int D = 32 * NJ, kLanes = D / 8, kHeads = 32 / kLanes;   // of a head; of a unit
   pdl_launch_dependents();
   pdl_wait_prior();
-  const int lane = threadIdx.x & 31, d0 = lane * E;
-  const int n_heads = p.q_heads + 2 * p.g.heads;
-  const long long item = (long long)blockIdx.x * kKvWarps + (threadIdx.x >> 5);
-  const int r = (int)(item / p.parts), h0 = (int)(item - (long long)r * p.parts) * p.per_warp;
-  const int h1 = min(h0 + p.per_warp, n_heads);
-  if (r >= p.b.n_rows) return;
-  const size_t x_at = (size_t)r * p.ldx + d0;
-  float next[E];
-  load_lane<E, F32>(p.x, x_at + (size_t)h0 * D, next);
-  float wq[E], wk[E];
+  const int lane = threadIdx.x, d0 = lane % kLanes * 8;
+  const int r = (int)(blockIdx.x / (unsigned)p.parts), part = (int)(blockIdx.x % (unsigned)p.parts);
+  const bool is_q = part < p.parts_q;
+  const int end = is_q ? p.q_heads : p.q_heads + 2 * p.g.heads;                      // past the last head of the kind
+  const int h0 = (is_q ? part : part - p.parts_q) * p.units * kHeads + (is_q ? 0 : p.q_heads);
+  const int units = min(p.units, (end - h0 + kHeads - 1) / kHeads);
+  // a lane past the last head works on that one and stores nothing
+  Raw8<F32> raw[kAppendUnits];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    wq[e] = p.q_norm && h0 < p.q_heads ? bf16_to_f32(p.q_norm[d0 + e]) : 1.f;
-    wk[e] = p.k_norm && h1 > p.q_heads ? bf16_to_f32(p.k_norm[d0 + e]) : 1.f;
-  }
+  for (int u = 0; u < kAppendUnits; ++u)
+    if (u < units) raw[u].load(p.x, (size_t)r * p.ldx + (size_t)min(h0 + u * kHeads + lane / kLanes, end - 1) * D + d0);
+  const uint16_t *norm = is_q ? p.q_norm : p.k_norm;
+  uint4 w = {};
+  if (norm) w = __ldcg(reinterpret_cast<const uint4 *>(norm + d0));
   int seq, pos;
   if (!kv_find_row(p.b, r, lane, seq, pos)) return;
-  RopeLane<E> rope;
-  rope.half = 0;
+  RopeLane rope;
+  rope.any = false;
   if (p.rope && pos >= 0 && h0 < p.q_heads + p.g.heads) {
     if (pos >= p.rope_rows) {
       if (lane == 0) atomicCAS(p.err, 0, kErrKvRange);
       return;
     }
-    rope.load(p.rope + (size_t)pos * p.rope_dim, p.rope_dim, p.interleaved, lane);
+    rope.load(p.rope + (size_t)pos * p.rope_dim, p.rope_dim, p.interleaved, lane, d0);
   }
-  uint8_t *page = h1 > p.q_heads && pos >= 0 ? kv_head_block(p.g, p.b, seq, pos, 0, p.err) : nullptr;
-  const int t = pos & (p.g.page - 1);
+  if (is_q) {
+#pragma unroll
+    for (int u = 0; u < kAppendUnits; ++u) {
+      if (u >= units) break;
+      float v[8];
+      raw[u].get(v);
+      norm_rope<kLanes, float>(v, true, norm != nullptr, w, p.eps, rope, p.interleaved, true);
+      const int h = h0 + u * kHeads + lane / kLanes;
+      if (h < end) *reinterpret_cast<uint4 *>(p.q_out + (size_t)r * p.ldq + h * D + d0) = bf16x8_rn(v);
+    }
+    return;
+  }
+  uint8_t *page = pos >= 0 ? kv_head_block(p.g, p.b, seq, pos, 0, p.err) : nullptr;
+  if (!page) return;
+  const int t = pos & (p.g.page - 1), j = d0 / 32, first_v = p.q_heads + p.g.heads;
 #pragma unroll 1
-  for (int h = h0; h < h1; ++h) {
-    float x[E];
+  for (int u = 0; u < units; ++u) {
+    const int h = h0 + u * kHeads + lane / kLanes;
+    const bool is_v = h >= first_v;
+    float v[8];
+    raw[0].get(v);
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = next[e];
-    if (h + 1 < h1) load_lane<E, F32>(p.x, x_at + (size_t)(h + 1) * D, next);
-    if (h < p.q_heads) {
-      norm_rope<E, float>(x, p.q_norm != nullptr, wq, p.eps, rope, p.interleaved, lane);
-      uint16_t *out = p.q_out + (size_t)r * p.ldq + h * D + d0;
-      uint32_t w[E / 2];
-#pragma unroll
-      for (int e = 0; e < E; e += 2)
-        w[e / 2] = f32_to_bf16_rne(x[e]) | ((uint32_t)f32_to_bf16_rne(x[e + 1]) << 16);
-      if constexpr (E == 4) *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
-      else *reinterpret_cast<uint32_t *>(out) = w[0];
-      continue;
-    }
-    if (!page) return;
-    const bool is_v = h >= p.q_heads + p.g.heads;
-    uint32_t code[E], param;
+    for (int i = 0; i + 1 < kAppendUnits; ++i) raw[i] = raw[i + 1];
+    uint32_t codes, param;
     bool fine;
-    if (is_v) {
-      fine = quantise_group<E, float>(x, code, param);
+    if (h0 + u * kHeads >= first_v) {                     // values only
+      fine = quantise_group<float>(v, codes, param);
     } else {
-      double k[E];
+      double k[8];
 #pragma unroll
-      for (int e = 0; e < E; ++e) k[e] = x[e];
-      norm_rope<E, double>(k, p.k_norm != nullptr, wk, p.eps, rope, p.interleaved, lane);
-      fine = quantise_group<E, double>(k, code, param);
+      for (int e = 0; e < 8; ++e) k[e] = v[e];
+      norm_rope<kLanes, double>(k, !is_v, norm != nullptr, w, p.eps, rope, p.interleaved, !is_v);
+      fine = quantise_group<double>(k, codes, param);
     }
+    if (h >= end) continue;
     if (!fine) atomicCAS(p.err, 0, kErrKvNonFinite);
-    uint8_t *blk = page + (size_t)(h - p.q_heads - (is_v ? p.g.heads : 0)) * p.g.head_bytes;
-    uint8_t *codes = blk + (is_v ? p.g.vc_off : 0) + t * (D / 2) + (is_v ? kv_v_byte(d0, NJ) : kv_k_byte(d0, NJ));
-    if constexpr (E == 4)
-      *reinterpret_cast<uint16_t *>(codes) = (uint16_t)(code[0] | (code[1] << 4) | (code[2] << 8) | (code[3] << 12));
-    else
-      *codes = (uint8_t)(code[0] | (code[1] << 4));
-    if (d0 % kKvGroup == 0)
-      reinterpret_cast<uint32_t *>(blk + (is_v ? p.g.vp_off : p.g.kp_off))[t * NJ + d0 / kKvGroup] = param;
+    uint8_t *blk = page + (size_t)(h - (is_v ? first_v : p.q_heads)) * p.g.head_bytes;
+    uint8_t *to = blk + (is_v ? p.g.vc_off : 0) + t * (D / 2) + (is_v ? kv_v_byte(d0, NJ) : kv_k_byte(d0, NJ));
+    if (is_v) {
+      *reinterpret_cast<uint16_t *>(to) = (uint16_t)codes;
+      *reinterpret_cast<uint16_t *>(to + 2 * NJ) = (uint16_t)(codes >> 16);
+    } else {
+      *reinterpret_cast<uint32_t *>(to) = codes;
+    }
+    if (d0 % kKvGroup == 0) reinterpret_cast<uint32_t *>(blk + (is_v ? p.g.vp_off : p.g.kp_off))[t * NJ + j] = param;
   }
 }
 
 // ------------------------------------------------------------------- read --
-// One warp per (row, kv head, K or V): min + scale * code in 32 bits (one
-// rounding: scale * code is exact), rounded to bf16.
-template <int E>
+// One warp per (row, K or V, 256 / D kv heads), 8 values a lane: min + scale *
+// code in 32 bits (one rounding: scale * code is exact), rounded to bf16.
+constexpr int kKvWarps = 8;
+
+template <int NJ>
 __global__ void __launch_bounds__(32 * kKvWarps)
-    rc_kv_read_kernel(const __grid_constant__ KvGeom g, const __grid_constant__ KvBatchDev b, uint16_t *k_out,
+    rc_kv_read_kernel(const __grid_constant__ KvGeom g, const __grid_constant__ KvBatchDev b, int parts, uint16_t *k_out,
                       uint16_t *v_out, int *err) {
-  constexpr int D = 32 * E, NJ = D / kKvGroup;
+  constexpr int D = 32 * NJ, kLanes = D / 8, kHeads = 32 / kLanes;
   pdl_launch_dependents();
   pdl_wait_prior();
-  const int lane = threadIdx.x & 31, d0 = lane * E;
+  const int lane = threadIdx.x & 31, d0 = lane % kLanes * 8;
   const long long item = (long long)blockIdx.x * kKvWarps + (threadIdx.x >> 5);
-  const int r = (int)(item / (2 * g.heads)), i = (int)(item - (long long)r * 2 * g.heads);
-  const int kv = i >= g.heads ? 1 : 0, h = i - kv * g.heads;
+  const int r = (int)(item / (2 * parts)), i = (int)(item - (long long)r * 2 * parts);
+  const bool is_v = i >= parts;
+  const int h = (is_v ? i - parts : i) * kHeads + lane / kLanes;
   if (r >= b.n_rows) return;
   int seq, pos;
-  if (!kv_find_row(b, r, lane, seq, pos)) return;
+  if (!kv_find_row(b, r, lane, seq, pos) || h >= g.heads) return;
   const uint8_t *blk = pos >= 0 ? kv_head_block(g, b, seq, pos, h, err) : nullptr;
   const int t = pos & (g.page - 1);
-  uint32_t w[E / 2];
+  float v[8];
 #pragma unroll
-  for (int e = 0; e < E / 2; ++e) w[e] = 0;
+  for (int e = 0; e < 8; ++e) v[e] = 0.f;
   if (blk) {
-    const uint8_t *codes = blk + (kv ? g.vc_off : 0) + t * (D / 2) + (kv ? kv_v_byte(d0, NJ) : kv_k_byte(d0, NJ));
-    const uint32_t par = __ldcg(reinterpret_cast<const uint32_t *>(blk + (kv ? g.vp_off : g.kp_off)) + t * NJ + d0 / kKvGroup);
-    uint32_t nib;
-    if constexpr (E == 4) nib = __ldcg(reinterpret_cast<const uint16_t *>(codes));
-    else nib = __ldcg(codes);
+    const uint8_t *at = blk + (is_v ? g.vc_off : 0) + t * (D / 2) + (is_v ? kv_v_byte(d0, NJ) : kv_k_byte(d0, NJ));
+    const uint32_t par = __ldcg(reinterpret_cast<const uint32_t *>(blk + (is_v ? g.vp_off : g.kp_off)) + t * NJ + d0 / kKvGroup);
+    const uint32_t codes = is_v ? __ldcg(reinterpret_cast<const uint16_t *>(at)) |
+                                      (uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(at + 2 * NJ)) << 16
+                                : __ldcg(reinterpret_cast<const uint32_t *>(at));
     const float sc = bf16_lo_f32(par), mn = bf16_hi_f32(par);
 #pragma unroll
-    for (int e = 0; e < E / 2; ++e) {
-      const float a = fmaf(sc, (float)(nib >> (8 * e) & 15), mn), c = fmaf(sc, (float)(nib >> (8 * e + 4) & 15), mn);
-      w[e] = f32_to_bf16_rne(a) | ((uint32_t)f32_to_bf16_rne(c) << 16);
-    }
+    for (int e = 0; e < 8; ++e) v[e] = fmaf(sc, (float)(codes >> (4 * e) & 15), mn);
   }
-  uint16_t *out = (kv ? v_out : k_out) + ((size_t)r * g.heads + h) * D + d0;
-  if constexpr (E == 4) *reinterpret_cast<uint2 *>(out) = make_uint2(w[0], w[1]);
-  else *reinterpret_cast<uint32_t *>(out) = w[0];
+  *reinterpret_cast<uint4 *>((is_v ? v_out : k_out) + ((size_t)r * g.heads + h) * D + d0) = bf16x8_rn(v);
 }
 
 // ------------------------------------------------------------- page moves --
@@ -480,9 +497,11 @@ int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, 
                q_heads * kv->dim);
   RC_CHECK_ARG(ldx % 8 == 0 && ldq % 8 == 0 && aligned16(x_dev) && aligned16(q_out_dev),
                "rc_kv_append: rows must start on 16-byte boundaries");
-  RC_CHECK_ARG(!rope_dev || (rope_rows >= 1 && rope_dim >= 8 && rope_dim <= kv->dim && rope_dim % 8 == 0),
-               "rc_kv_append: rope_dim %d must be a multiple of 8 up to head_dim (and rope_rows, %d, positive)", rope_dim,
+  RC_CHECK_ARG(!rope_dev || (rope_rows >= 1 && rope_dim >= 16 && rope_dim <= kv->dim && rope_dim % 16 == 0),
+               "rc_kv_append: rope_dim %d must be a multiple of 16 up to head_dim (and rope_rows, %d, positive)", rope_dim,
                rope_rows);
+  RC_CHECK_ARG(aligned16(rope_dev), "rc_kv_append: the rotation table must be 16-byte aligned");
+  RC_CHECK_ARG(aligned16(q_norm_dev) && aligned16(k_norm_dev), "rc_kv_append: norm weights must be 16-byte aligned");
   RC_CHECK_ARG(eps >= 0.f, "rc_kv_append: eps must not be negative");
   if (n_rows == 0 || n_seqs == 0) return RC_OK;
   RC_CUDA_TRY(cudaSetDevice(kv->ctx->device));
@@ -502,17 +521,18 @@ int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, 
   p.q_out = q_out_dev;
   p.ldq = ldq;
   p.err = kv->ctx->err;
-  // as many heads a warp as leave 64 warps an SM
-  const int heads = q_heads + 2 * kv->heads;
-  const long long spare = (long long)n_rows * heads / (64ll * kv->ctx->sm_count);
-  p.per_warp = spare < 1 ? 1 : spare < kAppendMaxHeads ? (int)spare : kAppendMaxHeads;
-  p.parts = (heads + p.per_warp - 1) / p.per_warp;
-  const long long blocks = ((long long)n_rows * p.parts + kKvWarps - 1) / kKvWarps;
+  // several units a warp where that leaves 16 warps an SM
+  const int unit = 256 / kv->dim, units_q = (q_heads + unit - 1) / unit, units_kv = (2 * kv->heads + unit - 1) / unit;
+  p.units = (long long)n_rows * (units_q + units_kv) >= 16ll * kAppendUnits * kv->ctx->sm_count ? kAppendUnits : 1;
+  p.parts_q = (units_q + p.units - 1) / p.units;
+  p.parts = p.parts_q + (units_kv + p.units - 1) / p.units;
+  const long long blocks = (long long)n_rows * p.parts;
   RC_CHECK_ARG(blocks <= INT_MAX, "rc_kv_append: too many rows (%d)", n_rows);
-  const dim3 grid((unsigned)blocks), block(32 * kKvWarps);
+  const dim3 grid((unsigned)blocks), block(32);
   const cudaStream_t s = pick_stream(kv->ctx, stream);
   const bool f32 = x_dtype == RC_DTYPE_F32;
-  if (kv->dim == 128) return f32 ? launch(rc_kv_append_kernel<4, true>, grid, block, s, p) : launch(rc_kv_append_kernel<4, false>, grid, block, s, p);
+  if (kv->dim == 128)
+    return f32 ? launch(rc_kv_append_kernel<4, true>, grid, block, s, p) : launch(rc_kv_append_kernel<4, false>, grid, block, s, p);
   return f32 ? launch(rc_kv_append_kernel<2, true>, grid, block, s, p) : launch(rc_kv_append_kernel<2, false>, grid, block, s, p);
 }
 
@@ -526,12 +546,13 @@ int rc_kv_read(rc_kv *kv, int layer, int n_rows, const int32_t *table_dev, int c
   RC_CUDA_TRY(cudaSetDevice(kv->ctx->device));
   const KvGeom g = kv_geom(kv, layer);
   const KvBatchDev b{table_dev, kv_len_dev, q_off_dev, cols, ld_table, n_seqs, n_rows};
-  const long long blocks = ((long long)n_rows * 2 * kv->heads + kKvWarps - 1) / kKvWarps;
+  const int unit = 256 / kv->dim, parts = (kv->heads + unit - 1) / unit;
+  const long long blocks = ((long long)n_rows * 2 * parts + kKvWarps - 1) / kKvWarps;
   RC_CHECK_ARG(blocks <= INT_MAX, "rc_kv_read: too many rows (%d)", n_rows);
   const dim3 grid((unsigned)blocks), block(32 * kKvWarps);
   const cudaStream_t s = pick_stream(kv->ctx, stream);
-  return kv->dim == 128 ? launch(rc_kv_read_kernel<4>, grid, block, s, g, b, k_out_dev, v_out_dev, kv->ctx->err)
-                        : launch(rc_kv_read_kernel<2>, grid, block, s, g, b, k_out_dev, v_out_dev, kv->ctx->err);
+  return kv->dim == 128 ? launch(rc_kv_read_kernel<4>, grid, block, s, g, b, parts, k_out_dev, v_out_dev, kv->ctx->err)
+                        : launch(rc_kv_read_kernel<2>, grid, block, s, g, b, parts, k_out_dev, v_out_dev, kv->ctx->err);
 }
 
 int rc_kv_move_pages(rc_kv *kv, const int32_t *src_dev, const int32_t *dst_dev, int n, int32_t *table_dev, int rows,
