@@ -19,7 +19,7 @@ namespace rc {
 // rounding boundary is off by a whole step), value heads are taken as they come;
 // the codes of both are found in 32 bits and those near a boundary once more in
 // 64.  A block is one warp, so that the room of a short one (queries) is free
-// before a long one (keys) ends: 4096 rows of 32 + 8 + 8 heads of 128 with their
+// before a long one (keys) ends: 4096 rows of 32 + 4 + 4 heads of 128 with their
 // read-back take 47 us, with blocks of two warps 50 and of eight 65.
 constexpr int kAppendUnits = 4, kAppendCtas = 24;
 
@@ -521,9 +521,11 @@ int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, 
   p.q_out = q_out_dev;
   p.ldq = ldq;
   p.err = kv->ctx->err;
-  // several units a warp where that leaves 16 warps an SM
+  // As many units a warp (4, 2 or 1) as leave 16 warps an SM.  4096 rows of 20 units (and their read-back): 47 us with
+  // 4, 57 with 2, 97 with 1; 859 rows of 8 units: 15.0, 11.5 and 12.7; 16 rows of 20 units: 9.2, 6.6 and 5.2.
   const int unit = 256 / kv->dim, units_q = (q_heads + unit - 1) / unit, units_kv = (2 * kv->heads + unit - 1) / unit;
-  p.units = (long long)n_rows * (units_q + units_kv) >= 16ll * kAppendUnits * kv->ctx->sm_count ? kAppendUnits : 1;
+  for (p.units = kAppendUnits; p.units > 1 && (long long)n_rows * (units_q + units_kv) < 16ll * p.units * kv->ctx->sm_count;)
+    p.units /= 2;
   p.parts_q = (units_q + p.units - 1) / p.units;
   p.parts = p.parts_q + (units_kv + p.units - 1) / p.units;
   const long long blocks = (long long)n_rows * p.parts;
