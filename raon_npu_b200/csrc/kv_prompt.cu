@@ -130,16 +130,6 @@ __device__ __forceinline__ void pr_ld32(uint32_t addr, uint32_t (&v)[32]) {
         "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(addr));
 }
-__device__ __forceinline__ void pr_st32(uint32_t addr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
 __device__ __forceinline__ void pr_st16(uint32_t addr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
@@ -249,11 +239,14 @@ __device__ __forceinline__ void pr_touch(uint32_t (&v)[32]) {   // nothing uses 
                  "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]),
                  "+r"(v[30]), "+r"(v[31]));
 }
-__device__ __forceinline__ void pr_scale8(uint32_t addr, float by) {
-  uint32_t v[8];
+__device__ __forceinline__ void pr_ld8(uint32_t addr, uint32_t *v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                : "r"(addr));
+}
+__device__ __forceinline__ void pr_scale8(uint32_t addr, float by) {
+  uint32_t v[8];
+  pr_ld8(addr, v);
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])
                :
@@ -364,8 +357,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
   if (warp < 8) {
     // ------------------------------------------------------------- softmax --
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPrRegsSoftmax));
-    const int t = warp >> 2, row = tid & (kPrRows - 1);
-    const uint32_t lane_at = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    // from a shuffle with a fixed lane, so that addresses and loop state are known to be the warp's and leave the
+    // threads' registers to the scores (spilled, the block loop takes a fifth longer)
+    const int wu = __shfl_sync(0xffffffffu, warp, 0), t = wu >> 2, row = tid & (kPrRows - 1);
+    const uint32_t lane_at = __shfl_sync(0xffffffffu, tmem, 0) + ((uint32_t)(32 * (wu & 3)) << 16);
     const uint32_t s_at = lane_at + L::s_col, p_at = lane_at + L::p_col + t * (kPrRows / 2), o_at = lane_at + L::o_col + t * D;
     const uint32_t bar_s = bars.s_full + 8 * t, bar_p = bars.p_full + 8 * t, bar_o = bars.o_done + 8 * t;
     int n = 0, done = 0;                                  // blocks of all items so far; this tile's
@@ -490,36 +485,50 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           const int flat = flat0 + row, qi = attn_row(p, flat);
           const bool live = qi < it->rows_do;
           uint16_t *dst = p.out + (size_t)(it->first + qi) * p.ldo + (size_t)(it->head * p.group + flat - qi * p.group) * D;
-          // columns 8W + 2i + o hold dim 32 (j + o) + 4 g + i, W = (g NJ + j) / 2; 32 columns cover 8 / NJ g's
-          constexpr int kPer = 8 / NJ;
           const float r = l == 0.f ? 0.f : 1.f / l, un = pow2f(-fv);
+          const unsigned long long mine = live ? reinterpret_cast<unsigned long long>(dst) : 0ull;
+          // columns 8W + 2i + o hold dim 32 (j + o) + 4 g + i, W = (g NJ + j) / 2; two of the 32-value groups at a time
 #pragma unroll 1
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t v[32];
+          for (int jj = 0; jj < NJ; jj += 2) {
+            uint32_t v[2][32];
             if (blocks) {
-              pr_ld32(o_at + 32 * i, v);
-              pr_wait_ld(v);
+#pragma unroll
+              for (int g = 0; g < 8; ++g) pr_ld8(o_at + 4 * (g * NJ + jj), &v[g / 4][8 * (g % 4)]);
+              pr_wait_ld(v[0]);
+              pr_touch(v[1]);
             } else {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = 0;
+              for (int e = 0; e < 32; ++e) v[0][e] = v[1][e] = 0;
             }
-            if (live) {
 #pragma unroll
-              for (int j = 0; j < NJ; ++j) {
-                const float bad = (nan_groups >> j) & 1 ? NAN : 0.f;
-                uint32_t w[2 * kPer];
+            for (int o = 0; o < 2; ++o) {
+              const float bad = (nan_groups >> (jj + o)) & 1 ? NAN : 0.f;
+              uint32_t u[4][4];                           // 16 bytes of the row each
 #pragma unroll
-                for (int g = 0; g < kPer; ++g) {
-                  const int c0 = 8 * ((g * NJ + j) / 2) + (j & 1);
-                  float x[4];
+              for (int g = 0; g < 8; ++g) {
+                float x[4];
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) x[e] = fmaf(__uint_as_float(v[c0 + 2 * e]) * r, un, bad);
-                  w[2 * g] = pack_bf16x2(x[0], x[1]);
-                  w[2 * g + 1] = pack_bf16x2(x[2], x[3]);
-                }
+                for (int e = 0; e < 4; ++e) x[e] = fmaf(__uint_as_float(v[g / 4][8 * (g % 4) + 2 * e + o]) * r, un, bad);
+                u[g / 2][2 * (g % 2)] = pack_bf16x2(x[0], x[1]);
+                u[g / 2][2 * (g % 2) + 1] = pack_bf16x2(x[2], x[3]);
+              }
+              // four lanes transpose their rows' quarters, so that a store writes 64 bytes of a row
 #pragma unroll
-                for (int g = 0; g < 2 * kPer; g += 4)
-                  *reinterpret_cast<uint4 *>(dst + 32 * j + 4 * kPer * i + 2 * g) = make_uint4(w[g], w[g + 1], w[g + 2], w[g + 3]);
+              for (int m = 1; m < 4; m *= 2)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                  if (!(x & m))
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                      const bool odd = lane & m;
+                      const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? u[x][e] : u[x + m][e], m);
+                      if (odd) u[x][e] = got;
+                      else u[x + m][e] = got;
+                    }
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+                const unsigned long long to = __shfl_sync(0xffffffffu, mine, (lane & 28) + m);
+                if (to) *reinterpret_cast<uint4 *>(to + 64 * (jj + o) + 16 * (lane & 3)) = make_uint4(u[m][0], u[m][1], u[m][2], u[m][3]);
               }
             }
           }
@@ -536,8 +545,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
   } else if (warp < 16) {
     // -------------------------------------------------- operands as f16 --
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPrRegsMake));
-    const int kv = (warp - 8) >> 2;                       // 0: K and tile 0's Q; 1: V and tile 1's Q
-    const int row = tid & (kPrRows - 1), w4 = warp & 3;
+    const int wu = __shfl_sync(0xffffffffu, warp, 0), kv = (wu - 8) >> 2;                       // 0: K and tile 0's Q; 1: V and tile 1's Q
+    const int row = tid & (kPrRows - 1), w4 = wu & 3;
     int *red = reinterpret_cast<int *>(sm + L::o_red) + 8 * kv;
     const uint32_t bar_full = (kv ? bars.v_full : bars.k_full), bar_empty = (kv ? bars.v_empty : bars.k_empty);
 
