@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
         const int pos = base + attn_row(p, flat0 + row);
         const int p_min = base + attn_row(p, min(flat0, last_flat));
         const int p_max = base + attn_row(p, min(flat0 + kPrRows - 1, last_flat));
-        float c_row = 0.f, ref = -INFINITY, l = 0.f;
+        float ref = -INFINITY, l = 0.f;
         int fv = 0;
         uint32_t nan_groups = 0;
         bool ok = true;
@@ -399,14 +399,10 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           pr_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bars.s_free);
-          if (j == 0) {
-            c_row = crow[(k & 1) * 2 * kPrRows + t * kPrRows + row];
-            if (c_row != c_row) c_row = 0.f, nan_groups = (1u << NJ) - 1u;
-          }
           ok = attn_wait(bars.v_info + 8 * ((n + j) % kPrInfo), (n + j) / kPrInfo & 1, abort, p.err);
           if (!ok) break;
           const int4 f = info[(n + j) % kPrInfo];
-          const float c = fmaxf(c_row * pow2f(-f.x), 0x1p-126f);   // above 0: a hidden score is -Inf
+          const float c = fmaxf(crow[(k & 1) * 2 * kPrRows + t * kPrRows + row] * pow2f(-f.x), 0x1p-126f);   // above 0 (also of NaN): a hidden score is -Inf
           const int c_hi = pos - t0, c_lo = p.window > 0 ? c_hi - p.window : INT_MIN, c_sink = p.sinks - t0;
           if (masked) {
 #pragma unroll
@@ -485,6 +481,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           const int flat = flat0 + row, qi = attn_row(p, flat);
           const bool live = qi < it->rows_do;
           uint16_t *dst = p.out + (size_t)(it->first + qi) * p.ldo + (size_t)(it->head * p.group + flat - qi * p.group) * D;
+          if (blocks && isnan(crow[(k & 1) * 2 * kPrRows + t * kPrRows + row])) nan_groups = (1u << NJ) - 1u;
           const float r = l == 0.f ? 0.f : 1.f / l, un = pow2f(-fv);
           const unsigned long long mine = live ? reinterpret_cast<unsigned long long>(dst) : 0ull;
           // columns 8W + 2i + o hold dim 32 (j + o) + 4 g + i, W = (g NJ + j) / 2; two of the 32-value groups at a time
