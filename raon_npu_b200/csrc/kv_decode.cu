@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
   constexpr int D = L::D, NC = L::cols;
   extern __shared__ __align__(128) uint8_t sm[];
   const AttnParams &a = p.a;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t bar_full = smem_addr(sm + L::o_bar), bar_empty = bar_full + 8 * L::stages;
   const uint32_t bar_item = bar_empty + 8 * L::stages, bar_taken = bar_item + 16;
   volatile int *abort = reinterpret_cast<volatile int *>(sm + L::o_flags);
@@ -355,8 +355,12 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
     }
     dc_sync();
     if (!*s_go) break;
-    const DcItem it = *reinterpret_cast<const DcItem *>(sm + L::o_item + 64 * (k & 1));
-    __syncwarp();
+    DcItem it = *reinterpret_cast<const DcItem *>(sm + L::o_item + 64 * (k & 1));
+    it.v0 = __shfl_sync(0xffffffffu, it.v0, 0), it.v1 = __shfl_sync(0xffffffffu, it.v1, 0), it.n_sink = __shfl_sync(0xffffffffu, it.n_sink, 0);
+    it.lo = __shfl_sync(0xffffffffu, it.lo, 0), it.len = __shfl_sync(0xffffffffu, it.len, 0), it.sinks = __shfl_sync(0xffffffffu, it.sinks, 0);
+    it.rows = __shfl_sync(0xffffffffu, it.rows, 0);
+    it.b = __shfl_sync(0xffffffffu, it.b, 0), it.head = __shfl_sync(0xffffffffu, it.head, 0), it.cb = __shfl_sync(0xffffffffu, it.cb, 0), it.chunk = __shfl_sync(0xffffffffu, it.chunk, 0), it.n_chunks = __shfl_sync(0xffffffffu, it.n_chunks, 0), it.first = __shfl_sync(0xffffffffu, it.first, 0), it.rows_do = __shfl_sync(0xffffffffu, it.rows_do, 0);
+
     if (lane == 0) mbar_arrive(bar_taken + 8 * (k & 1));
 
     if (it.b != cell_b || it.head != cell_head || it.cb != cell_cb) {
