@@ -3,7 +3,18 @@
 
 using namespace rc;
 
-// Rows of a sequence and kv head above which a call goes to the tensor-core kernel.
+// Rows of a sequence and kv head above which a call goes to the tensor-memory
+// kernel.  The decode kernel reads the cache once per 16 rows, split over as many
+// CTAs as there are; the other one once per 256, by one CTA a kv head.  Which is
+// faster turns on the number of sequences, and a row's bytes must not, so the rule
+// is on the rows alone, and where both sides lose alike.  us, decode / prompt, 4096
+// tokens, heads of 128:
+//                     1 sequence of 4 kv heads   of 16 kv heads   8 of 4 kv heads
+//    32 rows                  19.6 / 58.1          20.6 / 58.7       33.5 / 59.5
+//   128 rows                  20.6 / 58.7          59.1 / 59.4       95.2 / 60.7
+//   256 rows                  32.9 / 70.2          94.6 / 71.1      181.1 / 71.4
+//  1024 rows                  94.2 / 70.7                           705.1 / 75.8
+// The decode kernel also keeps weights below 2^-31 of the largest.
 constexpr long long kPromptRows = 255;
 
 extern "C" int rc_kv_attend(rc_kv *kv, int layer, const uint16_t *q_dev, int ldq, int q_heads, int n_rows,
