@@ -42,12 +42,14 @@ namespace rc {
 constexpr int kDcWarps = 4;                       // computing warps
 constexpr int kDcThreads = 32 * (kDcWarps + 1);   // and one that copies
 constexpr int kDcStage = 128;                     // tokens of a stage
-// A chunk is an eighth of the stages, but two to six of them (256 to 768
-// tokens: smaller ones cost more in partial results than they give in balance;
-// 64 sequences of up to 8191 tokens took 68.7 / 67.4 / 67.4 us with at most 4 /
-// 6 / 8, two of up to 131072 65.7 / 55.3 / 62.6 us), and a 256th where that is
-// more.
-constexpr int kDcMinStages = 2, kDcMaxStages = 6, kDcMaxChunks = 256;
+// A chunk is an eighth of the stages, but four to six of them (512 to 768
+// tokens: smaller ones cost more in partial results than they give in balance),
+// and a 256th where that is more.  us with at least 1 / 2 / 3 / 4 / 5: one
+// sequence of 333 tokens 8.9 / 9.2 / 8.1 / 7.9 / 7.9, 64 of up to 8191 tokens
+// 68.7 / 65.1 / 66.5 / 62.6 / 62.2, 32 that see 1028 tokens 21.6 / 21.8 / 21.2 /
+// 21.0 / 21.8 (one of 1024 takes 11.4 with 4 and 10.0 with 2); two of up to 131072
+// with at most 6 / 8 / 10: 54.0 / 60.8 / 56.9.
+constexpr int kDcMinStages = 4, kDcMaxStages = 6, kDcMaxChunks = 256;
 constexpr int kDcFan = 16;                        // partial results joined at a time
 constexpr int kDcGroups = (kDcMaxChunks + kDcFan - 1) / kDcFan;
 
