@@ -62,7 +62,7 @@ struct PrLayout {
   static constexpr int o_crow = o_red + 64;                       // [2 items][256] score scales, NaN for a row that is
   static constexpr int o_item = o_crow + 2 * 2 * kPrRows * 4;     // [2] items
   static constexpr int o_bar = o_item + 2 * 64;
-  static constexpr int n_bars = 33 + 2 * kPrRaw;
+  static constexpr int n_bars = 29 + 2 * kPrRaw;
   static constexpr int o_misc = o_bar + 8 * n_bars;               // tensor memory address, abort word
   static constexpr int o_prefix = o_misc + 16;                    // [n_seqs / 32 + 1] items of the sequences before
   static constexpr int o_raw = (o_prefix + (kKvMaxSeqs / 32 + 1) * 4 + 127) / 128 * 128;
@@ -219,7 +219,7 @@ __device__ __forceinline__ uint32_t pr_chunk(int r, int c) {
 }
 
 struct PrBars {
-  uint32_t item_full, item_empty, q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_empty, drain, vote, s_free, v_info, raw_full, raw_empty;
+  uint32_t item_full, item_empty, q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_empty, drain, vote, s_free, raw_full, raw_empty;
 };
 
 // Of columns 32 k .. 32 k + 31, those a row sees: column <= c_hi, and > c_lo or < c_sink.
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t bar0 = smem_addr(sm + L::o_bar);
   const PrBars bars{bar0,       bar0 + 16,  bar0 + 32,  bar0 + 48,  bar0 + 64,  bar0 + 80, bar0 + 96,
-                    bar0 + 112, bar0 + 128, bar0 + 144, bar0 + 160, bar0 + 176, bar0 + 192, bar0 + 208, bar0 + 224, bar0 + 232, bar0 + 264, bar0 + 264 + 8 * kPrRaw};
+                    bar0 + 112, bar0 + 128, bar0 + 144, bar0 + 160, bar0 + 176, bar0 + 192, bar0 + 208, bar0 + 224, bar0 + 232, bar0 + 232 + 8 * kPrRaw};
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + L::o_misc);
   volatile int *abort = reinterpret_cast<volatile int *>(sm + L::o_misc + 4);
   int4 *info = reinterpret_cast<int4 *>(sm + L::o_info);
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
       mbar_init(bars.item_empty + 8 * s, 19);            // softmax, operands, copies, scores, values
       mbar_init(bars.q_full + 8 * s, kPrRows);
       mbar_init(bars.q_empty + 8 * s, 1);
-      mbar_init(bars.k_full + 8 * s, kPrRows);
+      mbar_init(bars.k_full + 8 * s, kPrRows + 4);   // K's rows, and V's exponent from four warps
       mbar_init(bars.k_empty + 8 * s, 1);
       mbar_init(bars.v_full + 8 * s, kPrRows);
       mbar_init(bars.v_empty + 8 * s, 1);
@@ -318,7 +318,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
     mbar_init(bars.vote, 4);
     mbar_init(bars.vote + 8, 4);
     mbar_init(bars.s_free, 4);
-    for (int s = 0; s < kPrInfo; ++s) mbar_init(bars.v_info + 8 * s, 4);
     for (int s = 0; s < kPrRaw; ++s) {
       mbar_init(bars.raw_full + 8 * s, 1);
       mbar_init(bars.raw_empty + 8 * s, 4);
@@ -399,8 +398,6 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           pr_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bars.s_free);
-          ok = attn_wait(bars.v_info + 8 * ((n + j) % kPrInfo), (n + j) / kPrInfo & 1, abort, p.err);
-          if (!ok) break;
           const int4 f = info[(n + j) % kPrInfo];
           const float c = fmaxf(crow[(k & 1) * 2 * kPrRows + t * kPrRows + row] * pow2f(-f.x), 0x1p-126f);   // above 0 (also of NaN): a hidden score is -Inf
           const int c_hi = pos - t0, c_lo = p.window > 0 ? c_hi - p.window : INT_MIN, c_sink = p.sinks - t0;
@@ -639,10 +636,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           poison[((n % kPrInfo) * 2 + kv) * kPrRows + row] = (uint8_t)mask;
           if (row == 0) *(reinterpret_cast<int2 *>(info + n % kPrInfo) + kv) = make_int2(f, bad);
         };
-        if (kv) {                                         // the softmax threads wait for V's exponent by itself
+        if (kv) {
+          // K's barrier waits for it too, so that the scores' one tells the softmax of both.  The barrier is at this
+          // block or the one two before it at most: with three packed slots K's last block has been made by now.
+          static_assert(kPrRaw <= 3, "V two blocks ahead of K");
           tell();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bars.v_info + 8 * (n % kPrInfo));
+          if (lane == 0) mbar_arrive(bars.k_full + 8 * s);
         }
         if (!attn_wait(bar_empty + 8 * s, ((n >> 1) & 1) ^ 1, abort, p.err)) break;
         if (!kv) tell();                                  // not before: block n - 4's may still be read
