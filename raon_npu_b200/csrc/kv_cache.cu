@@ -34,7 +34,8 @@ struct AppendParams {
   int rope_rows, rope_dim, interleaved;
   uint16_t *q_out;
   int ldq;
-  int units, parts_q, parts;   // units of a warp; warps for the queries of a row, for the row
+  int units_q, units_kv;       // units of a warp
+  int parts_q, parts;          // warps for the queries of a row, for the row
   int *err;
 };
 
@@ -192,8 +193,9 @@ __global__ void __launch_bounds__(32, kAppendCtas) rc_kv_append_kernel(const __g
   const int r = (int)(blockIdx.x / (unsigned)p.parts), part = (int)(blockIdx.x % (unsigned)p.parts);
   const bool is_q = part < p.parts_q;
   const int end = is_q ? p.q_heads : p.q_heads + 2 * p.g.heads;                      // past the last head of the kind
-  const int h0 = (is_q ? part : part - p.parts_q) * p.units * kHeads + (is_q ? 0 : p.q_heads);
-  const int units = min(p.units, (end - h0 + kHeads - 1) / kHeads);
+  const int per = is_q ? p.units_q : p.units_kv;
+  const int h0 = (is_q ? part : part - p.parts_q) * per * kHeads + (is_q ? 0 : p.q_heads);
+  const int units = min(per, (end - h0 + kHeads - 1) / kHeads);
   // a lane past the last head works on that one and stores nothing
   Raw8<F32> raw[kAppendUnits];
 #pragma unroll
@@ -521,13 +523,15 @@ int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, 
   p.q_out = q_out_dev;
   p.ldq = ldq;
   p.err = kv->ctx->err;
-  // As many units a warp (4, 2 or 1) as leave 16 warps an SM.  4096 rows of 20 units (and their read-back): 47 us with
-  // 4, 57 with 2, 97 with 1; 859 rows of 8 units: 15.0, 11.5 and 12.7; 16 rows of 20 units: 9.2, 6.6 and 5.2.
+  // As many units of queries a warp (4, 2 or 1) as leave 16 warps an SM, and half as many of keys and values, which take
+  // longer.  4096 rows of 20 units (and their read-back): 47 us with 4, 57 with 2, 97 with 1; 859 rows of 8 units: 15.0,
+  // 11.5 and 12.7; 16 rows of 20 units: 9.2, 6.6 and 5.2.  The halves took 1.7, 0.7 and 0 us off.
   const int unit = 256 / kv->dim, units_q = (q_heads + unit - 1) / unit, units_kv = (2 * kv->heads + unit - 1) / unit;
-  for (p.units = kAppendUnits; p.units > 1 && (long long)n_rows * (units_q + units_kv) < 16ll * p.units * kv->ctx->sm_count;)
-    p.units /= 2;
-  p.parts_q = (units_q + p.units - 1) / p.units;
-  p.parts = p.parts_q + (units_kv + p.units - 1) / p.units;
+  for (p.units_q = kAppendUnits; p.units_q > 1 && (long long)n_rows * (units_q + units_kv) < 16ll * p.units_q * kv->ctx->sm_count;)
+    p.units_q /= 2;
+  p.units_kv = p.units_q > 1 ? p.units_q / 2 : 1;
+  p.parts_q = (units_q + p.units_q - 1) / p.units_q;
+  p.parts = p.parts_q + (units_kv + p.units_kv - 1) / p.units_kv;
   const long long blocks = (long long)n_rows * p.parts;
   RC_CHECK_ARG(blocks <= INT_MAX, "rc_kv_append: too many rows (%d)", n_rows);
   const dim3 grid((unsigned)blocks), block(32);

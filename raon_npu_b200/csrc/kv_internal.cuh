@@ -1,6 +1,8 @@
 // Definitions shared by the KV cache translation units: the pool's geometry,
 // the batch description and the arithmetic of one cached row.
 #pragma once
+#include <limits.h>
+
 
 #include "rc_device.cuh"
 #include "rc_internal.cuh"
@@ -67,18 +69,22 @@ __device__ __forceinline__ bool kv_find_row(const KvBatchDev &b, int r, int lane
     pos = __ldcg(b.kv_len + r) - 1;
     return true;
   }
-  int below = 0;   // offsets <= r
+  int last_len = 0;                 // of the window before
   for (int k0 = 0; k0 <= b.n_seqs; k0 += 32) {
-    const int k = k0 + lane;
-    const unsigned m = __ballot_sync(0xffffffffu, k <= b.n_seqs && __ldcg(b.q_off + k) <= r);
-    below += __popc(m);
-    if (m != 0xffffffffu) break;
+    const int k = k0 + lane, off = k <= b.n_seqs ? __ldcg(b.q_off + k) : INT_MAX, len = k < b.n_seqs ? __ldcg(b.kv_len + k) : 0;
+    const unsigned m = __ballot_sync(0xffffffffu, k <= b.n_seqs && off <= r);
+    if (m != 0xffffffffu) {
+      const int n = __popc(m);      // offsets of this window <= r
+      seq = k0 + n - 1;
+      if (seq < 0 || seq >= b.n_seqs) return false;
+      const int hi = __shfl_sync(0xffffffffu, off, n);
+      pos = __shfl_sync(0xffffffffu, len, (n - 1) & 31);
+      pos = (n ? pos : last_len) - hi + r;
+      return true;
+    }
+    last_len = __shfl_sync(0xffffffffu, len, 31);
   }
-  seq = below - 1;
-  if (seq < 0 || seq >= b.n_seqs) return false;
-  const int lo = __ldcg(b.q_off + seq), hi = __ldcg(b.q_off + seq + 1);
-  pos = __ldcg(b.kv_len + seq) - (hi - lo) + (r - lo);
-  return true;
+  return false;
 }
 
 // Head block of (page of position pos, head); null, with the error word set,
