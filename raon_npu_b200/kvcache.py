@@ -33,6 +33,7 @@ from .device import CUDA_STREAM_LEGACY, Context, _ptr
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _BF16 = frozenset((torch.bfloat16, torch.int16, torch.uint16))   # bf16 values, or their bits
 _F32 = frozenset((torch.float32,))
+_float32 = torch.float32
 
 
 def rope_table(positions: int, rope_dim: int, base: float = 10000.0) -> np.ndarray:
@@ -51,9 +52,11 @@ def _ints(t, ndim: int, what: str):
 
 def _rows(t, width: int, what: str, dev: int, types=_BF16):
     """(rows, row stride in elements) of [rows, width] or [rows, heads, head_dim] values."""
+    shape = t.shape
+    if len(shape) == 2 and shape[1] == width and t.is_contiguous() and t.dtype in types and t.get_device() == dev:
+        return shape[0], width
     if t.dtype not in types or t.get_device() != dev:
         raise ValueError(f"{what} must be a {'bf16' if types is _BF16 else 'f32'} tensor on cuda:{dev}, got {t.dtype} on {t.device}")
-    shape = t.shape
     if len(shape) == 2:
         inner = shape[1] == width and (t.is_contiguous() or width == 1 or t.stride(1) == 1)
     elif len(shape) == 3:
@@ -110,7 +113,7 @@ class KvCache:
 
     def __init__(self, ctx: Context, layers: int, kv_heads: int, head_dim: int, pages: int, page_size: int = 64,
                  pool=None):
-        self.ctx, self.lib = ctx, ctx.lib
+        self.ctx, self.lib, self.device = ctx, ctx.lib, ctx.device
         self.layers, self.kv_heads, self.head_dim = int(layers), int(kv_heads), int(head_dim)
         self.pages, self.page_size = int(pages), int(page_size)
         self.scale = self.head_dim ** -0.5
@@ -148,17 +151,22 @@ class KvCache:
         except Exception:
             pass
 
+    def _norm(self, w, name: str) -> int:
+        if w.dtype in _BF16 and w.get_device() == self.device and w.numel() == self.head_dim and w.is_contiguous():
+            return w.data_ptr()
+        raise ValueError(f"{name} must hold {self.head_dim} bf16 values on the device")
+
     def _batch_args(self, batch: KvBatch, rows: int, what: str):
         q_off = batch.q_off
-        if batch.table.get_device() != self.ctx.device:
-            raise ValueError(f"{what}: the batch is on {batch.table.device}, the cache on cuda:{self.ctx.device}")
+        if batch.table.get_device() != self.device:
+            raise ValueError(f"{what}: the batch is on {batch.table.device}, the cache on cuda:{self.device}")
         if q_off is None and rows != batch.n_seqs:
             raise ValueError(f"{what}: {rows} rows for {batch.n_seqs} sequences without q_off")
         return batch.table.data_ptr(), batch.kv_len.data_ptr(), None if q_off is None else q_off.data_ptr()
 
     def _stream(self, stream) -> int:
         """The stream to launch on; torch's default stream is the legacy one (0 is the context's own in the C ABI)."""
-        return int(stream) if stream is not None else _raw_stream(self.ctx.device) or CUDA_STREAM_LEGACY
+        return int(stream) if stream is not None else _raw_stream(self.device) or CUDA_STREAM_LEGACY
 
     # ---------------------------------------------------------- operators --
     def append(self, layer: int, x, batch: KvBatch, q_out=None, q_heads: int = 0, q_norm=None, k_norm=None,
@@ -170,8 +178,8 @@ class KvCache:
         the query and key heads (None: no norm).  rope f32 [positions,
         rope_dim]: cos | sin of every position (None: no rotation)."""
         width = (q_heads + 2 * self.kv_heads) * self.head_dim
-        dev = self.ctx.device
-        f32 = x.dtype is torch.float32
+        dev = self.device
+        f32 = x.dtype is _float32
         rows, ldx = _rows(x, width, "x", dev, _F32 if f32 else _BF16)
         ldq = 0
         if q_heads:
@@ -180,20 +188,17 @@ class KvCache:
             n, ldq = _rows(q_out, q_heads * self.head_dim, "q_out", dev)
             if n != rows:
                 raise ValueError(f"append: x has {rows} rows, q_out {n}")
-        for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-            if w is not None and (w.dtype not in _BF16 or w.get_device() != dev or w.numel() != self.head_dim or
-                                  not w.is_contiguous()):
-                raise ValueError(f"{name} must hold {self.head_dim} bf16 values on the device")
+        q_w = None if q_norm is None else self._norm(q_norm, "q_norm")
+        k_w = None if k_norm is None else self._norm(k_norm, "k_norm")
         rope_rows = rope_dim = 0
         if rope is not None:
-            if rope.dtype is not torch.float32 or rope.dim() != 2 or rope.get_device() != dev or not rope.is_contiguous():
+            if rope.dtype is not _float32 or rope.dim() != 2 or rope.get_device() != dev or not rope.is_contiguous():
                 raise ValueError(f"rope must be a contiguous f32 tensor [positions, rope_dim] on cuda:{dev}")
             rope_rows, rope_dim = rope.shape
         table, kv_len, q_off = self._batch_args(batch, rows, "append")
         rc = self.lib.rc_kv_append(
             self.handle, layer, x.data_ptr(), _lib.RC_DTYPE_F32 if f32 else _lib.RC_DTYPE_BF16, ldx, q_heads, rows,
-            table, batch.columns, batch.ld, kv_len, q_off, batch.n_seqs, None if q_norm is None else q_norm.data_ptr(),
-            None if k_norm is None else k_norm.data_ptr(), eps, None if rope is None else rope.data_ptr(), rope_rows,
+            table, batch.columns, batch.ld, kv_len, q_off, batch.n_seqs, q_w, k_w, eps, None if rope is None else rope.data_ptr(), rope_rows,
             rope_dim, 1 if interleaved else 0, q_out.data_ptr() if q_heads else None, ldq, self._stream(stream))
         if rc:
             check(rc, "rc_kv_append")
@@ -205,7 +210,7 @@ class KvCache:
         scale: of the scores (default 1 / sqrt(head_dim)).  window > 0: a row
         sees itself, the window - 1 tokens before it and the first ``sinks``
         tokens of its sequence; 0: every token up to itself."""
-        dev = self.ctx.device
+        dev = self.device
         shape = q.shape
         width = shape[1] if len(shape) == 2 else shape[1] * shape[2] if len(shape) == 3 else 0
         heads = width // self.head_dim
@@ -224,8 +229,8 @@ class KvCache:
     def read(self, layer: int, batch: KvBatch, k_out, v_out, stream: int | None = None) -> None:
         """The cached keys and values of the batch's rows in bf16: k_out, v_out [rows, kv_heads, head_dim], contiguous."""
         width = self.kv_heads * self.head_dim
-        rows, ldk = _rows(k_out, width, "k_out", self.ctx.device)
-        n, ldv = _rows(v_out, width, "v_out", self.ctx.device)
+        rows, ldk = _rows(k_out, width, "k_out", self.device)
+        n, ldv = _rows(v_out, width, "v_out", self.device)
         if n != rows or ldk != width or ldv != width:
             raise ValueError("read: k_out and v_out must be contiguous and of one shape")
         table, kv_len, q_off = self._batch_args(batch, rows, "read")
