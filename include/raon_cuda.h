@@ -414,9 +414,10 @@ int rc_kv_destroy(rc_kv *kv);
  * multiple of 16, at most head_dim.  Queries go to q_out [n_rows][ldq] bf16;
  * keys and values are quantised (the group rule of rc_quantize_q4nx: bf16
  * floor of the minimum, bf16 ceiling of (max - min) / 15 stepped up until it
- * covers the maximum, nearest code, ties to even), in 64 bits throughout, and
- * stored at the row's position.  A group with a non-finite value or a range
- * that overflows is stored as NaN and sets the device error word. */
+ * covers the maximum, nearest code, ties to even), with the bytes of a 64-bit
+ * computation, and stored at the row's position.  A group with a non-finite
+ * value or a range that overflows is stored as NaN and sets the device error
+ * word.  x, q_out, the norm weights and rope are 16-byte aligned. */
 int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, int q_heads, int n_rows,
                  const int32_t *table_dev, int cols, int ld_table, const int32_t *kv_len_dev,
                  const int32_t *q_off_dev, int n_seqs, const uint16_t *q_norm_dev, const uint16_t *k_norm_dev, float eps,
@@ -429,9 +430,14 @@ int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, 
  * row at position p sees: all of them when window == 0, else those with
  * t > p - window or t < sinks.  out [n_rows][ldo] bf16; zeros where a row sees
  * nothing.  ldq and ldo are multiples of 8 and both buffers 16-byte aligned.
- * A row's bytes do not depend on the other sequences of the batch.  Scratch
- * grows on the first call for a larger batch or table (that call
- * synchronises the device). */
+ * At most 256 query heads share a kv head, and max_q * q_heads / kv_heads is
+ * at most 2^24.  A row's bytes do not depend on the other sequences of the
+ * batch, for one max_q: up to 255 rows (max_q * q_heads / kv_heads) a kernel
+ * that keeps every weight, above it one that takes weights below 2^-31 of the
+ * largest as zero.  Values are rounded to 11 bits or more before the products;
+ * scores, sums and results are 32-bit.  Scratch grows on the first call for a
+ * larger batch or table (that call synchronises the device) and belongs to the
+ * context: keep its calls on one stream at a time. */
 int rc_kv_attend(rc_kv *kv, int layer, const uint16_t *q_dev, int ldq, int q_heads, int n_rows,
                  const int32_t *table_dev, int cols, int ld_table, const int32_t *kv_len_dev,
                  const int32_t *q_off_dev, int n_seqs, int max_q, float scale, int window, int sinks, uint16_t *out_dev, int ldo,

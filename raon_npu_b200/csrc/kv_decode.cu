@@ -33,6 +33,12 @@
 // a stage each.  A row of one chunk is written directly; else each chunk leaves
 // (maximum, sum, values) in scratch and the last one to arrive joins them in
 // chunk order.
+//
+// Measured (32 query heads, 4 kv heads of 128): 64 sequences of 65 to 8191 tokens
+// 62.6 us (170 MB: 2.7 TB/s, 42% of the copy rate), two of 111870 and 131072 tokens
+// 53.8 us (156 MB, 45%), one of 333 tokens 7.9 us.  Bound by instruction issue: 0.51
+// a cycle from 13 warps an SM, which is what the registers allow; the unpacking of
+// the codes is about half of it.
 #include <limits.h>
 
 #include "kv_attn.cuh"

@@ -29,6 +29,16 @@
 //
 // A V group that holds NaN is zero in the product and reaches the rows that
 // see its token by hand, so that 0 * NaN does not reach the others.
+//
+// Measured: 4096 rows of 32 heads over 4 kv heads of 128, causal, 140 us: 982
+// TFLOP/s of visible pairs, 59% of the matrix peak; chunks of 2048 and 1416 rows of
+// 32 heads over 8 that see 4096 tokens and 16 sinks 227 us (62%); six prompts of 117
+// to 701 tokens, 16 heads of 64, 27 us.  Bound by the chain of a block: scores (640
+// cycles), their way into registers (300), maximum (500), weights (1700; without the
+// exponentials the prompt took 125 us, without making K and V 132, with half the
+// products 141), values (530).  S and P in one place, and S for each tile, was
+// slower (188 us): then a tile's chain has no overlap.  A short prompt pays 7 us
+// before its first score: items, rows, codes.
 #include <limits.h>
 
 #include "kv_attn.cuh"
@@ -637,8 +647,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           if (row == 0) *(reinterpret_cast<int2 *>(info + n % kPrInfo) + kv) = make_int2(f, bad);
         };
         if (kv) {
-          // K's barrier waits for it too, so that the scores' one tells the softmax of both.  The barrier is at this
-          // block or the one two before it at most: with three packed slots K's last block has been made by now.
+          // K's barrier waits for it too, so that the scores' one tells the softmax of both.  It is in this block's
+          // phase: V's packed block n takes the slot of K's n - 1, so K's n - 2 has been made.
           static_assert(kPrRaw <= 3, "V two blocks ahead of K");
           tell();
           __syncwarp();
