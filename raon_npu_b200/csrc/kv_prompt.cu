@@ -386,15 +386,17 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
         const int pos = base + attn_row(p, flat0 + row);
         const int p_min = base + attn_row(p, min(flat0, last_flat));
         const int p_max = base + attn_row(p, min(flat0 + kPrRows - 1, last_flat));
+        // blocks clear_lo .. clear_hi - 1 are seen whole by every row of the tile
+        const int skip = it->blk_lo - it->sink_blocks;
+        const int clear_lo = p.window <= 0 ? 0 : max(it->sink_blocks, (max(p_max - p.window, -1) + kPrRows) / kPrRows - skip);
+        const int clear_hi = (p_min + 1) / kPrRows - skip;
         float ref = -INFINITY, l = 0.f;
         int fv = 0;
         uint32_t nan_groups = 0;
         bool ok = true;
 #pragma unroll 1
         for (int j = 0; j < blocks; ++j, ++done) {
-          const int t0 = pr_block(*it, j);
-          const bool masked = !(t0 + kPrRows - 1 <= p_min &&
-                                (p.window <= 0 || t0 > p_max - p.window || t0 + kPrRows <= p.sinks));
+          const bool masked = j < clear_lo || j >= clear_hi;
           ok = attn_wait(bar_s, done & 1, abort, p.err);
           if (!ok) break;
           pr_fence_after();
@@ -410,6 +412,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           if (lane == 0) mbar_arrive(bars.s_free);
           const int4 f = info[(n + j) % kPrInfo];
           const float c = fmaxf(crow[(k & 1) * 2 * kPrRows + t * kPrRows + row] * pow2f(-f.x), 0x1p-126f);   // above 0 (also of NaN): a hidden score is -Inf
+          const int t0 = pr_block(*it, j);
           const int c_hi = pos - t0, c_lo = p.window > 0 ? c_hi - p.window : INT_MIN, c_sink = p.sinks - t0;
           if (masked) {
 #pragma unroll
