@@ -78,6 +78,7 @@ struct AttnParams {
   int window, sinks;
   uint16_t *out;
   int ldo;
+  int *turns;            // of the cache
   int *err;
 };
 

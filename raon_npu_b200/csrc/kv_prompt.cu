@@ -15,7 +15,8 @@
 // have a P each, and a tile's next scores are there when its softmax comes for
 // them.  CTAs are persistent and every role goes straight from one item to the
 // next, so the next item's query rows and blocks come in while the last one's
-// results go out.  The loops of the other roles are rolled and short on purpose:
+// results go out.  Items after the first are claimed by turns (dealt in fixed
+// rounds, six ragged prompts took 28 us for 20, and one of 4096 139 for 141).  The loops of the other roles are rolled and short on purpose:
 // together with a larger text they outgrew the instruction cache, and each of
 // them, the issuing warp first, ran at the speed of its misses.
 //
@@ -30,10 +31,10 @@
 // A V group that holds NaN is zero in the product and reaches the rows that
 // see its token by hand, so that 0 * NaN does not reach the others.
 //
-// Measured: 4096 rows of 32 heads over 4 kv heads of 128, causal, 140 us: 982
+// Measured: 4096 rows of 32 heads over 4 kv heads of 128, causal, 141 us: 977
 // TFLOP/s of visible pairs, 59% of the matrix peak; chunks of 2048 and 1416 rows of
-// 32 heads over 8 that see 4096 tokens and 16 sinks 227 us (62%); six prompts of 117
-// to 701 tokens, 16 heads of 64, 27 us.  Bound by the chain of a block: scores (640
+// 32 heads over 8 that see 4096 tokens and 16 sinks 229 us (62%); six prompts of 117
+// to 701 tokens, 16 heads of 64, 20 us.  Bound by the chain of a block: scores (640
 // cycles), their way into registers (300), maximum (500), weights (1700; without the
 // exponentials the prompt took 125 us, without making K and V 132, with half the
 // products 141), values (530).  S and P in one place, and S for each tile, was
@@ -72,7 +73,7 @@ struct PrLayout {
   static constexpr int o_crow = o_red + 64;                       // [2 items][256] score scales, NaN for a row that is
   static constexpr int o_item = o_crow + 2 * 2 * kPrRows * 4;     // [2] items
   static constexpr int o_bar = o_item + 2 * 64;
-  static constexpr int n_bars = 29 + 2 * kPrRaw;
+  static constexpr int n_bars = 30 + 2 * kPrRaw;
   static constexpr int o_misc = o_bar + 8 * n_bars;               // tensor memory address, abort word
   static constexpr int o_prefix = o_misc + 16;                    // [n_seqs / 32 + 1] items of the sequences before
   static constexpr int o_raw = (o_prefix + (kKvMaxSeqs / 32 + 1) * 4 + 127) / 128 * 128;
@@ -199,11 +200,6 @@ __device__ __forceinline__ PrItem pr_item(const AttnParams &p, const int *prefix
 // Token t is visible to a row of the item.
 __device__ __forceinline__ bool pr_seen_by_item(const PrItem &it, int t) { return t < it.len && (t >= it.lo || t < it.sinks); }
 
-// The k-th item of this CTA: rounds over the grid, every second one backwards, which evens out falling costs.
-__device__ __forceinline__ int pr_turn(int k) {
-  return k * (int)gridDim.x + (k & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
-}
-
 // Exponents of a token's params: the larger of the scales' and of minima more than 2^19 times as large.
 template <int NJ>
 __device__ __forceinline__ int pr_exponent(const uint32_t (&par)[NJ]) {
@@ -229,7 +225,7 @@ __device__ __forceinline__ uint32_t pr_chunk(int r, int c) {
 }
 
 struct PrBars {
-  uint32_t item_full, item_empty, q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_empty, drain, vote, s_free, raw_full, raw_empty;
+  uint32_t item_full, item_empty, q_full, q_empty, k_full, k_empty, v_full, v_empty, s_full, p_full, o_done, o_empty, drain, vote, s_free, claim, raw_full, raw_empty;
 };
 
 // Of columns 32 k .. 32 k + 31, those a row sees: column <= c_hi, and > c_lo or < c_sink.
@@ -300,7 +296,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t bar0 = smem_addr(sm + L::o_bar);
   const PrBars bars{bar0,       bar0 + 16,  bar0 + 32,  bar0 + 48,  bar0 + 64,  bar0 + 80, bar0 + 96,
-                    bar0 + 112, bar0 + 128, bar0 + 144, bar0 + 160, bar0 + 176, bar0 + 192, bar0 + 208, bar0 + 224, bar0 + 232, bar0 + 232 + 8 * kPrRaw};
+                    bar0 + 112, bar0 + 128, bar0 + 144, bar0 + 160, bar0 + 176, bar0 + 192, bar0 + 208, bar0 + 224, bar0 + 232, bar0 + 240, bar0 + 240 + 8 * kPrRaw};
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + L::o_misc);
   volatile int *abort = reinterpret_cast<volatile int *>(sm + L::o_misc + 4);
   int4 *info = reinterpret_cast<int4 *>(sm + L::o_info);
@@ -328,6 +324,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
     mbar_init(bars.vote, 4);
     mbar_init(bars.vote + 8, 4);
     mbar_init(bars.s_free, 4);
+    mbar_init(bars.claim, 1);
     for (int s = 0; s < kPrRaw; ++s) {
       mbar_init(bars.raw_full + 8 * s, 1);
       mbar_init(bars.raw_empty + 8 * s, 4);
@@ -695,7 +692,13 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
 #pragma unroll 1
       for (int k = 0;; ++k) {
         if (!attn_wait(bars.item_empty + 8 * (k & 1), ((k >> 1) & 1) ^ 1, abort, p.err)) break;
-        const int i = pr_turn(k);
+        // the first item by the CTA's number, the next ones by turns, claimed when the last one's copies are on their way
+        int i = blockIdx.x;
+        if (k > 0) {
+          if (!attn_wait(bars.claim, (k - 1) & 1, abort, p.err)) break;
+          if (lane == 0) i = (int)gridDim.x + atomicAdd(p.turns, 1);
+          i = __shfl_sync(0xffffffffu, i, 0);
+        }
         PrItem it;
         it.b = -1;
         if (i < total) it = pr_item(p, prefix, i, lane);
@@ -706,6 +709,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
         __syncwarp();
         if (i >= total) break;
       }
+      // no claim comes after a CTA's last: the last CTA to get here leaves the counters at zero
+      if (lane == 0 && atomicAdd(p.turns + 1, 1) == (int)gridDim.x - 1) p.turns[0] = p.turns[1] = 0;
     } else if (warp == 18) {
       // ------------------------------------------------- packed K and V --
       const uint32_t part = p.g.head_bytes / 2;           // K or V of a page
@@ -737,6 +742,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
                                   bars.raw_full + 8 * slot);
           }
         }
+        if (lane == 0) mbar_arrive(bars.claim);
       }
       // copies in flight land before the CTA leaves: the last phase of each slot that had one, with a limit
       for (int i = max(0, h - kPrRaw); i < h; ++i) mbar_wait_bounded_warp(bars.raw_full + 8 * (i % kPrRaw), i / kPrRaw & 1);
