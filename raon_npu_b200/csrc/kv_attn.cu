@@ -52,7 +52,7 @@ extern "C" int rc_kv_attend(rc_kv *kv, int layer, const uint16_t *q_dev, int ldq
   p.sinks = sinks;
   p.out = out_dev;
   p.ldo = ldo;
-  p.turns = kv->turns;
+  p.turns = kv->ctx->attn_turns;
   p.err = kv->ctx->err;
   const cudaStream_t s = pick_stream(kv->ctx, stream);
   return (long long)p.max_q * p.group > kPromptRows ? kv_attend_prompt(kv->ctx, p, s) : kv_attend_decode(kv->ctx, p, p.max_q, s);

@@ -78,7 +78,7 @@ struct AttnParams {
   int window, sinks;
   uint16_t *out;
   int ldo;
-  int *turns;            // of the cache
+  int *turns;            // items claimed by a prompt call, CTAs that are done; zero between calls
   int *err;
 };
 

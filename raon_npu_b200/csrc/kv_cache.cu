@@ -474,14 +474,6 @@ int rc_kv_create(rc_ctx *ctx, int layers, int pages, int kv_heads, int head_dim,
     }
     kv->owned = 1;
   }
-  cudaError_t e = cudaMalloc(&kv->turns, 2 * sizeof(int));
-  if (e == cudaSuccess) e = cudaMemset(kv->turns, 0, 2 * sizeof(int));
-  if (e == cudaSuccess) e = cudaDeviceSynchronize();   // calls may go to streams that do not wait for this one
-  if (e != cudaSuccess) {
-    rc_kv_destroy(kv);
-    set_error("rc_kv_create: %s", cudaGetErrorString(e));
-    return RC_ERR_CUDA;
-  }
   *out = kv;
   return RC_OK;
 }
@@ -489,9 +481,10 @@ int rc_kv_create(rc_ctx *ctx, int layers, int pages, int kv_heads, int head_dim,
 int rc_kv_destroy(rc_kv *kv) {
   if (!kv) return RC_OK;
   cudaSetDevice(kv->ctx->device);
-  cudaDeviceSynchronize();   // calls may sit on caller streams
-  if (kv->owned) cudaFree(kv->pool);
-  cudaFree(kv->turns);
+  if (kv->owned) {
+    cudaDeviceSynchronize();   // calls may sit on caller streams
+    cudaFree(kv->pool);
+  }
   free(kv);
   return RC_OK;
 }

@@ -13,7 +13,6 @@ struct rc_kv {
   uint8_t *pool;
   int owned;             // the pool is this cache's own allocation
   size_t head_bytes, page_bytes, layer_bytes;
-  int *turns;            // device: items claimed by a prompt call, CTAs that are done; zero between calls
 };
 
 namespace rc {

@@ -98,6 +98,10 @@ int report_error_word(rc_ctx *ctx, int word) {
       return RC_ERR_INVALID;
     }
     ++ctx->timeout_epoch;
+    // what a call that gave up has left of the counts that are zero between calls
+    RC_CUDA_TRY(cudaMemset(ctx->attn_turns, 0, 2 * sizeof(int)));
+    if (ctx->attn_count) RC_CUDA_TRY(cudaMemset(ctx->attn_count, 0, ctx->attn_count_cap * sizeof(int)));
+    RC_CUDA_TRY(cudaDeviceSynchronize());
     set_error("a kernel gave up a bounded wait (device error word %d)", word);
     return RC_ERR_TIMEOUT;
   }
@@ -182,6 +186,9 @@ int rc_init(int device, rc_ctx **out) {
   if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking);
   if (e == cudaSuccess) e = cudaMalloc(&ctx->err, sizeof(int));
   if (e == cudaSuccess) e = cudaMemset(ctx->err, 0, sizeof(int));
+  if (e == cudaSuccess) e = cudaMalloc(&ctx->attn_turns, 2 * sizeof(int));
+  if (e == cudaSuccess) e = cudaMemset(ctx->attn_turns, 0, 2 * sizeof(int));
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();   // launches may go to streams that do not wait for this one
   if (e == cudaSuccess) e = cudaMalloc(&ctx->qflag, sizeof(int));
   if (e == cudaSuccess) {
     size_t warps = (size_t)ctx->sm_count * kGemvMaxWarps;   // stream-K partials: one slot pair per warp
@@ -206,6 +213,7 @@ int rc_destroy(rc_ctx *ctx) {
   cudaFree(ctx->bf_partials);
   cudaFree(ctx->counters);
   cudaFree(ctx->err);
+  cudaFree(ctx->attn_turns);
   cudaFree(ctx->qflag);
   cudaFree(ctx->dev_x);
   cudaFree(ctx->dev_y);

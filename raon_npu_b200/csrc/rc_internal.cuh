@@ -121,6 +121,7 @@ struct rc_ctx {
   void *attn_part;
   size_t attn_part_cap;
   int *attn_count;
+  int *attn_turns;      // [2], zero between calls
   size_t attn_count_cap;
 };
 
