@@ -20,7 +20,7 @@ namespace rc {
 // before a long one (keys) ends: with the read-back below, 4096 rows of 32 + 4 + 4
 // heads of 128 took 47 us so, with blocks of two warps 50 and of eight 65.
 // Measured: those rows in 30 us (86 MB in and out: 2.9 TB/s, 45% of the copy rate)
-// and 12 for the read-back; 16 rows of a decode step in 5.2 us with it.  Bound by
+// and 10 for the read-back; 16 rows of a decode step in 5.2 us with it.  Bound by
 // instruction issue (0.60 a cycle with 19 warps an SM; 250 for a unit of 256
 // values) and, with few rows, by four dependent loads: the row's sequence, its page
 // and rotation, the values.
@@ -267,10 +267,11 @@ __global__ void __launch_bounds__(32, kAppendCtas) rc_kv_append_kernel(const __g
 }
 
 // ------------------------------------------------------------------- read --
-// One warp per (row, K or V, 256 / D kv heads), 8 values a lane: min + scale *
+// One warp per (row, 256 / D kv heads), K and V, 8 values a lane: min + scale *
 // code in 32 bits (one rounding: scale * code is exact), rounded to bf16.  4096
-// rows of 4 + 4 heads of 128 take 12 us (10.5 MB), a third of it the launch and the
-// loads that depend on one another; blocks of one warp made it 19.
+// rows of 4 + 4 heads of 128 take 10 us (10.5 MB), most of it the launch and three
+// loads that depend on one another; with a warp each for K and V it took 12, with
+// blocks of one warp 19.
 constexpr int kKvWarps = 8;
 
 template <int NJ>
@@ -282,28 +283,29 @@ __global__ void __launch_bounds__(32 * kKvWarps)
   pdl_wait_prior();
   const int lane = threadIdx.x & 31, d0 = lane % kLanes * 8;
   const long long item = (long long)blockIdx.x * kKvWarps + (threadIdx.x >> 5);
-  const int r = (int)(item / (2 * parts)), i = (int)(item - (long long)r * 2 * parts);
-  const bool is_v = i >= parts;
-  const int h = (is_v ? i - parts : i) * kHeads + lane / kLanes;
+  const int r = (int)(item / parts), h = (int)(item - (long long)r * parts) * kHeads + lane / kLanes;
   if (r >= b.n_rows) return;
   int seq, pos;
   if (!kv_find_row(b, r, lane, seq, pos) || h >= g.heads) return;
   const uint8_t *blk = pos >= 0 ? kv_head_block(g, b, seq, pos, h, err) : nullptr;
   const int t = pos & (g.page - 1);
-  float v[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  uint32_t par[2] = {0, 0}, codes[2] = {0, 0};   // zeros for a row that is empty or outside
   if (blk) {
-    const uint8_t *at = blk + (is_v ? g.vc_off : 0) + t * (D / 2) + (is_v ? kv_v_byte(d0, NJ) : kv_k_byte(d0, NJ));
-    const uint32_t par = __ldcg(reinterpret_cast<const uint32_t *>(blk + (is_v ? g.vp_off : g.kp_off)) + t * NJ + d0 / kKvGroup);
-    const uint32_t codes = is_v ? __ldcg(reinterpret_cast<const uint16_t *>(at)) |
-                                      (uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(at + 2 * NJ)) << 16
-                                : __ldcg(reinterpret_cast<const uint32_t *>(at));
-    const float sc = bf16_lo_f32(par), mn = bf16_hi_f32(par);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = fmaf(sc, (float)(codes >> (4 * e) & 15), mn);
+    const uint8_t *k = blk + t * (D / 2) + kv_k_byte(d0, NJ), *v = blk + g.vc_off + t * (D / 2) + kv_v_byte(d0, NJ);
+    const int at = t * NJ + d0 / kKvGroup;
+    par[0] = __ldcg(reinterpret_cast<const uint32_t *>(blk + g.kp_off) + at);
+    par[1] = __ldcg(reinterpret_cast<const uint32_t *>(blk + g.vp_off) + at);
+    codes[0] = __ldcg(reinterpret_cast<const uint32_t *>(k));
+    codes[1] = __ldcg(reinterpret_cast<const uint16_t *>(v)) | (uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(v + 2 * NJ)) << 16;
   }
-  *reinterpret_cast<uint4 *>((is_v ? v_out : k_out) + ((size_t)r * g.heads + h) * D + d0) = bf16x8_rn(v);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float sc = bf16_lo_f32(par[i]), mn = bf16_hi_f32(par[i]);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaf(sc, (float)(codes[i] >> (4 * e) & 15), mn);
+    *reinterpret_cast<uint4 *>((i ? v_out : k_out) + ((size_t)r * g.heads + h) * D + d0) = bf16x8_rn(x);
+  }
 }
 
 // ------------------------------------------------------------- page moves --
@@ -560,7 +562,7 @@ int rc_kv_read(rc_kv *kv, int layer, int n_rows, const int32_t *table_dev, int c
   const KvGeom g = kv_geom(kv, layer);
   const KvBatchDev b{table_dev, kv_len_dev, q_off_dev, cols, ld_table, n_seqs, n_rows};
   const int unit = 256 / kv->dim, parts = (kv->heads + unit - 1) / unit;
-  const long long blocks = ((long long)n_rows * 2 * parts + kKvWarps - 1) / kKvWarps;
+  const long long blocks = ((long long)n_rows * parts + kKvWarps - 1) / kKvWarps;
   RC_CHECK_ARG(blocks <= INT_MAX, "rc_kv_read: too many rows (%d)", n_rows);
   const dim3 grid((unsigned)blocks), block(32 * kKvWarps);
   const cudaStream_t s = pick_stream(kv->ctx, stream);
