@@ -168,6 +168,13 @@ class KvCache:
         """The stream to launch on; torch's default stream is the legacy one (0 is the context's own in the C ABI)."""
         return int(stream) if stream is not None else _raw_stream(self.device) or CUDA_STREAM_LEGACY
 
+    def _torch_stream(self, handle: int):
+        """The torch stream of a handle as the C ABI takes it (0: the context's own)."""
+        dev = torch.device("cuda", self.device)
+        if handle == CUDA_STREAM_LEGACY:
+            return torch.cuda.default_stream(dev)
+        return torch.cuda.ExternalStream(handle or self.ctx.stream, dev)
+
     # ---------------------------------------------------------- operators --
     def append(self, layer: int, x, batch: KvBatch, q_out=None, q_heads: int = 0, q_norm=None, k_norm=None,
                eps: float = 1e-6, rope=None, interleaved: bool = False, stream: int | None = None) -> None:
@@ -314,6 +321,9 @@ class KvCache:
         if moves:
             dev = torch.device("cuda", self.ctx.device)
             m = torch.tensor(moves, dtype=torch.int32).t().contiguous().to(dev)
+            if stream is not None:
+                # the ids live on the current stream and are dropped here, maybe long before ``stream`` gets to them
+                m.record_stream(self._torch_stream(int(stream)))
             self.move_pages(m[0], m[1], stream=stream)
 
 
