@@ -436,8 +436,10 @@ int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, 
  * that keeps every weight, above it one that takes weights below 2^-31 of the
  * largest as zero.  Values are rounded to 11 bits or more before the products;
  * scores, sums and results are 32-bit.  Scratch grows on the first call for a
- * larger batch or table (that call synchronises the device) and belongs to the
- * context: keep its calls on one stream at a time. */
+ * larger batch or table (that call allocates and synchronises the device, so it
+ * must come before the call is captured) and belongs to the context: keep its
+ * calls on one stream at a time.  Scratch that a captured call uses lives as
+ * long as the context, whatever later calls need. */
 int rc_kv_attend(rc_kv *kv, int layer, const uint16_t *q_dev, int ldq, int q_heads, int n_rows,
                  const int32_t *table_dev, int cols, int ld_table, const int32_t *kv_len_dev,
                  const int32_t *q_off_dev, int n_seqs, int max_q, float scale, int window, int sinks, uint16_t *out_dev, int ldo,

@@ -72,6 +72,8 @@ static int grow_device(void **p, size_t *cap, size_t need) {
   return RC_OK;
 }
 
+static int clear_attn_counts(rc_ctx *ctx);
+
 // The status of an error word read back from the device (cleared when set).
 int report_error_word(rc_ctx *ctx, int word) {
   if (word) {
@@ -98,10 +100,8 @@ int report_error_word(rc_ctx *ctx, int word) {
       return RC_ERR_INVALID;
     }
     ++ctx->timeout_epoch;
-    // what a call that gave up has left of the counts that are zero between calls
-    RC_CUDA_TRY(cudaMemset(ctx->attn_turns, 0, 2 * sizeof(int)));
-    if (ctx->attn_count) RC_CUDA_TRY(cudaMemset(ctx->attn_count, 0, ctx->attn_count_cap * sizeof(int)));
-    RC_CUDA_TRY(cudaDeviceSynchronize());
+    int rc = clear_attn_counts(ctx);
+    if (rc) return rc;
     set_error("a kernel gave up a bounded wait (device error word %d)", word);
     return RC_ERR_TIMEOUT;
   }
@@ -119,26 +119,61 @@ int ensure_sample_scratch(rc_ctx *ctx, size_t bytes) {
   return grow_device(&ctx->sample_bits, &ctx->sample_bits_cap, bytes);
 }
 
-// Scratch of one attention call: grows only, after the whole device is idle.
-int ensure_attn_scratch(rc_ctx *ctx, size_t bytes, size_t counters) {
-  if (bytes > ctx->attn_part_cap) {
-    RC_CUDA_TRY(cudaDeviceSynchronize());
-    int rc = grow_device(&ctx->attn_part, &ctx->attn_part_cap, bytes);
-    if (rc) return rc;
+// Scratch that launches keep the address of.  A captured graph may hold the old
+// block, so it stays on ctx->outgrown until the context goes; a new one is at
+// least twice as large, so what stays is never more than what is in use.
+// ``counts``: words that are zero between launches.  Growth allocates and
+// synchronises, so it must not happen inside stream capture.
+static int grow_kept(rc_ctx *ctx, void **p, size_t *cap, size_t need, bool counts) {
+  if (need <= *cap) return RC_OK;
+  rc_outgrown *old = static_cast<rc_outgrown *>(calloc(1, sizeof(rc_outgrown)));
+  if (!old) {
+    set_error("out of host memory");
+    return RC_ERR_CUDA;
   }
-  if (counters > ctx->attn_count_cap) {
-    RC_CUDA_TRY(cudaDeviceSynchronize());
-    int *c = nullptr;
-    RC_CUDA_TRY(cudaMalloc(&c, counters * sizeof(int)));
-    cudaError_t e = cudaMemset(c, 0, counters * sizeof(int));
+  size_t bytes = need > 2 * *cap ? need : 2 * *cap;
+  void *block = nullptr;
+  cudaError_t e = cudaMalloc(&block, bytes);
+  if (e == cudaErrorMemoryAllocation && bytes > need) {
+    cudaGetLastError();
+    bytes = need;
+    e = cudaMalloc(&block, bytes);
+  }
+  if (e == cudaSuccess && counts) {
+    e = cudaMemset(block, 0, bytes);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();   // the launch may go to a stream that does not wait for this one
-    if (e != cudaSuccess) cudaFree(c);
-    RC_CUDA_TRY(e);
-    if (ctx->attn_count) cudaFree(ctx->attn_count);
-    ctx->attn_count = c;
-    ctx->attn_count_cap = counters;
+    if (e != cudaSuccess) cudaFree(block);
   }
+  if (e != cudaSuccess) {
+    free(old);
+    set_error("scratch of %zu bytes: %s", need, cudaGetErrorString(e));
+    return RC_ERR_CUDA;
+  }
+  old->block = *p;
+  old->bytes = *cap;
+  old->counts = counts;
+  old->next = ctx->outgrown;
+  ctx->outgrown = old;
+  *p = block;
+  *cap = bytes;
   return RC_OK;
+}
+
+// What a call that gave up has left of the counts that are zero between calls, also those that a graph may hold.
+static int clear_attn_counts(rc_ctx *ctx) {
+  RC_CUDA_TRY(cudaDeviceSynchronize());                  // of no call that still counts
+  RC_CUDA_TRY(cudaMemset(ctx->attn_turns, 0, 2 * sizeof(int)));
+  if (ctx->attn_count) RC_CUDA_TRY(cudaMemset(ctx->attn_count, 0, ctx->attn_count_cap));
+  for (rc_outgrown *o = ctx->outgrown; o; o = o->next)
+    if (o->counts && o->block) RC_CUDA_TRY(cudaMemset(o->block, 0, o->bytes));
+  RC_CUDA_TRY(cudaDeviceSynchronize());
+  return RC_OK;
+}
+
+// Scratch of one attention call.
+int ensure_attn_scratch(rc_ctx *ctx, size_t bytes, size_t counters) {
+  int rc = grow_kept(ctx, &ctx->attn_part, &ctx->attn_part_cap, bytes, false);
+  return rc ? rc : grow_kept(ctx, reinterpret_cast<void **>(&ctx->attn_count), &ctx->attn_count_cap, counters * sizeof(int), true);
 }
 
 int ensure_host_staging(rc_ctx *ctx, size_t xb, size_t yb) {
@@ -220,6 +255,11 @@ int rc_destroy(rc_ctx *ctx) {
   cudaFree(ctx->sample_bits);
   cudaFree(ctx->attn_part);
   cudaFree(ctx->attn_count);
+  while (rc_outgrown *o = ctx->outgrown) {
+    ctx->outgrown = o->next;
+    cudaFree(o->block);
+    free(o);
+  }
   if (ctx->pin_x) cudaFreeHost(ctx->pin_x);
   if (ctx->pin_y) cudaFreeHost(ctx->pin_y);
   if (ctx->pin_err) cudaFreeHost(ctx->pin_err);

@@ -91,6 +91,14 @@ struct rc_weight {
   float *bias;         // optional f32 [n] on the device
 };
 
+// A block of scratch that a captured graph may still use.
+struct rc_outgrown {
+  void *block;
+  size_t bytes;
+  bool counts;   // words that are zero between launches
+  rc_outgrown *next;
+};
+
 struct rc_ctx {
   int device;
   int sm_count;
@@ -119,10 +127,11 @@ struct rc_ctx {
   size_t sample_bits_cap;
   // Attention scratch: chunk partials and, zero between launches, arrival counters.
   void *attn_part;
-  size_t attn_part_cap;
+  size_t attn_part_cap;   // bytes
   int *attn_count;
-  int *attn_turns;      // [2], zero between calls
-  size_t attn_count_cap;
+  size_t attn_count_cap;  // bytes
+  int *attn_turns;        // [2], zero between calls
+  rc_outgrown *outgrown;  // blocks that larger ones have replaced
 };
 
 namespace rc {

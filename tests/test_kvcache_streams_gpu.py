@@ -60,3 +60,35 @@ def test_page_copies_wait_for_their_stream(torch, ctx, kind, op):  # noqa: F811
         pool.data[:, d] = pool.data[:, s]
     assert np.array_equal(dev.cpu().numpy(), pool.data)
     assert all((o == 11).all() for o in others)
+
+
+@pytest.mark.parametrize("d,hq,heads", [(128, 8, 2), (64, 24, 2)])
+def test_captured_calls_outlive_the_growth_of_scratch(torch, ctx, d, hq, heads):  # noqa: F811
+    """Batches of 1, 2, 4 and 8 sequences captured in that order, on tables that widen: every one asks for more scratch
+    than the last, and the earlier graphs go on giving their bytes without touching anybody else's memory."""
+    from raon_npu_b200.device import Context
+    own = Context(0)                                       # with no scratch yet
+    graphs = []
+    for i, n in enumerate((1, 2, 4, 8)):
+        c = Case(torch, own, d, heads, 16, [1500 + 17 * k for k in range(n)], seed=n, extra_cols=2 + 400 * i, layers=1)
+        c.layer = 0
+        q = torch.randn((n, hq, d), device="cuda").bfloat16()
+        out = torch.zeros_like(q)
+        c.cache.attend(0, q, c.batch, out)                 # grows what it needs
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c.cache.attend(0, q, c.batch, out)
+        graphs.append((graph, out, out.clone(), c, q))
+    torch.cuda.empty_cache()
+    others = [torch.full((1 << k,), 0x5A, dtype=torch.uint8, device="cuda") for k in range(9, 26) for _ in range(3)]
+    for _ in range(2):
+        for graph, out, want, _, _ in graphs:
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+    own.sync()
+    assert all((o == 0x5A).all() for o in others)
+    del graphs, graph
+    own.close()
