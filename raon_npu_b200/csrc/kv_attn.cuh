@@ -109,6 +109,12 @@ __device__ __forceinline__ void attn_seq(const AttnParams &p, int b, int &first,
   if (bad) atomicCAS(p.err, 0, kErrKvRange);
 }
 
+// First token of the window of the row at ``pos``, which may be negative (an
+// empty row) and the window anything up to the largest int: no sum of the two.
+__device__ __forceinline__ int attn_window_lo(const AttnParams &p, int pos) {
+  return p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
+}
+
 // Values d .. d+3 of query column ``flat`` (row * group + head in the group)
 // of a sequence: acc / sum, zeros when nothing was seen.
 __device__ __forceinline__ void attn_write4(const AttnParams &p, int first, int rows_do, int flat, int head, int D, int d,

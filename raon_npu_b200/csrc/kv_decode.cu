@@ -78,7 +78,7 @@ struct DcSeq {
 __device__ __forceinline__ DcSeq dc_seq(const AttnParams &p, int b) {
   DcSeq s;
   attn_seq(p, b, s.first, s.rows, s.rows_do, s.len);
-  s.lo = p.window > 0 ? max(0, s.len - s.rows - p.window + 1) : 0;
+  s.lo = attn_window_lo(p, s.len - s.rows);
   s.sinks = p.window > 0 ? min(p.sinks, s.lo) : 0;
   const int first = s.lo / kDcStage;
   s.n_sink = min((s.sinks + kDcStage - 1) / kDcStage, first);

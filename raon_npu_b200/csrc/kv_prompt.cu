@@ -189,7 +189,7 @@ __device__ __forceinline__ PrItem pr_item(const AttnParams &p, const int *prefix
   const int base = it.len - it.rows;                                   // position of row 0
   const int p_first = base + attn_row(p, it.flat0);
   const int p_last = base + min(it.rows_do - 1, attn_row(p, it.flat0 + 2 * kPrRows - 1));
-  it.lo = p.window > 0 ? max(0, p_first - p.window + 1) : 0;
+  it.lo = attn_window_lo(p, p_first);
   it.sinks = p.window > 0 ? min(p.sinks, it.lo) : 0;
   it.blk_lo = it.lo / kPrRows;
   it.sink_blocks = min((it.sinks + kPrRows - 1) / kPrRows, it.blk_lo);
