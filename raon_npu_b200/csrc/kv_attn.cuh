@@ -116,16 +116,15 @@ __device__ __forceinline__ int attn_window_lo(const AttnParams &p, int pos) {
 }
 
 // Values d .. d+3 of query column ``flat`` (row * group + head in the group)
-// of a sequence: acc / sum, zeros when nothing was seen.
+// of a sequence.
 __device__ __forceinline__ void attn_write4(const AttnParams &p, int first, int rows_do, int flat, int head, int D, int d,
-                                            float4 acc, float sum) {
+                                            float4 v) {
   const int qi = attn_row(p, flat);
   if (qi >= rows_do) return;
-  const float r = sum == 0.f ? 0.f : 1.f / sum;
   uint16_t *dst = p.out + (size_t)(first + qi) * p.ldo + (head * p.group + flat - qi * p.group) * D + d;
   *reinterpret_cast<uint2 *>(dst) =
-      make_uint2(f32_to_bf16_rne(acc.x * r) | ((uint32_t)f32_to_bf16_rne(acc.y * r) << 16),
-                 f32_to_bf16_rne(acc.z * r) | ((uint32_t)f32_to_bf16_rne(acc.w * r) << 16));
+      make_uint2(f32_to_bf16_rne(v.x) | ((uint32_t)f32_to_bf16_rne(v.y) << 16),
+                 f32_to_bf16_rne(v.z) | ((uint32_t)f32_to_bf16_rne(v.w) << 16));
 }
 
 int kv_attend_decode(rc_ctx *ctx, const AttnParams &a, int max_q, cudaStream_t s);   // kv_decode.cu

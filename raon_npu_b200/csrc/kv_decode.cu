@@ -198,7 +198,8 @@ __device__ __forceinline__ bool dc_arrive_last(int *count, int n, volatile int *
   return *s_last;
 }
 
-// Joins n <= kDcFan partial results in order; sink(column, value, 4 sums, reference, sum).
+// Joins n <= kDcFan partial results, each a mean of values with the reference and sum of its weights, in order;
+// sink(column, value, 4 means, reference, sum).
 template <int NJ, int NB, typename Sink>
 __device__ __forceinline__ void dc_join(const float *src, int n, float *scratch, int tid, Sink sink) {
   constexpr int D = 32 * NJ, NC = 8 * NB;
@@ -217,13 +218,17 @@ __device__ __forceinline__ void dc_join(const float *src, int n, float *scratch,
       v[c] = c < n ? __ldcg(reinterpret_cast<const float4 *>(src + c * kSlot + (size_t)col * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
     float top = -INFINITY, sum = 0.f;
     for (int c = 0; c < n; ++c) top = fmaxf(top, ml[c * NC + col].x);
+    const auto weight = [&](int c) {
+      const float2 x = ml[c * NC + col];
+      return (top == -INFINITY ? 1.f : exp2f(x.x - top)) * x.y;
+    };
+    for (int c = 0; c < n; ++c) sum += weight(c);
+    const float r = sum == 0.f ? 0.f : 1.f / sum;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int c = 0; c < kDcFan; ++c) {
       if (c >= n) break;
-      const float2 x = ml[c * NC + col];
-      const float f = top == -INFINITY ? 1.f : exp2f(x.x - top);
-      sum = fmaf(f, x.y, sum);
+      const float f = weight(c) * r;
       acc.x = fmaf(f, v[c].x, acc.x), acc.y = fmaf(f, v[c].y, acc.y), acc.z = fmaf(f, v[c].z, acc.z), acc.w = fmaf(f, v[c].w, acc.w);
     }
     sink(col, d, acc, top, sum);
@@ -708,7 +713,8 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
       if (++slot == L::stages) slot = 0, phase ^= 1;
     }
 
-    // ---- this warp's share to shared memory
+    // ---- this warp's share to shared memory, divided by its weights: these are up to 2^15 each, and their sum of values
+    // near the largest number has no 32-bit form
     const float un0 = pow2f(-(fexp >> 1)), un1 = pow2f(-(fexp - (fexp >> 1)));
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -719,10 +725,11 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, x);
         if (g == 0) s_m[warp * NC + col] = m[nb][c], s_l[warp * NC + col] = ls;
+        const float r = ls == 0.f ? 0.f : 1.f / ls;
 #pragma unroll
         for (int j = 0; j < 2 * NJ; ++j)
           *reinterpret_cast<float2 *>(s_o + (warp * NC + col) * D + 32 * (j / 2) + 4 * g + 2 * (j % 2)) =
-              make_float2(o[nb][j][c] * un0 * un1, o[nb][j][2 + c] * un0 * un1);
+              make_float2(o[nb][j][c] * r * un0 * un1, o[nb][j][2 + c] * r * un0 * un1);
       }
     dc_sync();
 
@@ -734,16 +741,22 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
       float top = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kDcWarps; ++w) top = fmaxf(top, s_m[w * NC + col]);
+      float fl[kDcWarps];
+#pragma unroll
+      for (int w = 0; w < kDcWarps; ++w) {
+        fl[w] = (top == -INFINITY ? 1.f : exp2f(s_m[w * NC + col] - top)) * s_l[w * NC + col];
+        sum += fl[w];
+      }
+      const float r = sum == 0.f ? 0.f : 1.f / sum;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kDcWarps; ++w) {
-        const float mw = s_m[w * NC + col], f = mw == top && top == -INFINITY ? 1.f : exp2f(mw - top);
+        const float f = fl[w] * r;
         const float4 v = *reinterpret_cast<const float4 *>(s_o + (w * NC + col) * D + d);
-        sum = fmaf(f, s_l[w * NC + col], sum);
         acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
       }
       if (it.n_chunks == 1) {
-        attn_write4(a, it.first, it.rows_do, it.cb * NC + col, it.head, D, d, acc, sum);
+        attn_write4(a, it.first, it.rows_do, it.cb * NC + col, it.head, D, d, acc);
       } else {
         float *dst = p.part + (cell * p.slots + it.chunk) * kSlot;
         __stcg(reinterpret_cast<float4 *>(dst + (size_t)col * D + d), acc);
@@ -760,7 +773,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
         const int n = min(kDcFan, it.n_chunks - grp * kDcFan);
         if (groups == 1) {
           dc_join<NJ, NB>(src, n, s_o, tid, [&](int col, int d, float4 acc, float top, float sum) {
-            attn_write4(a, it.first, it.rows_do, it.cb * NC + col, it.head, D, d, acc, sum);
+            attn_write4(a, it.first, it.rows_do, it.cb * NC + col, it.head, D, d, acc);
           });
         } else {
           float *mid = cell_part + (size_t)(p.slots - kDcGroups) * kSlot;
@@ -771,7 +784,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
           });
           if (dc_arrive_last(count, groups, s_last, tid))
             dc_join<NJ, NB>(mid, groups, s_o, tid, [&](int col, int d, float4 acc, float top, float sum) {
-              attn_write4(a, it.first, it.rows_do, it.cb * NC + col, it.head, D, d, acc, sum);
+              attn_write4(a, it.first, it.rows_do, it.cb * NC + col, it.head, D, d, acc);
             });
         }
       }
