@@ -171,7 +171,7 @@ struct DcLayout {
   static constexpr int stage = kDcStage * D * 5 / 4;
   static constexpr int stages = NJ == 4 ? (NB == 1 ? 2 : 3) : (NB == 1 ? 5 : 6);
   static constexpr int join = kDcWarps * cols * D * 4;                       // the warps' values of one item
-  static_assert(join >= cols * kDcFan * 8, "the joined parts' (reference, sum) lie there too");
+  static_assert(join >= cols * kDcFan * 12, "the joined parts' (reference, sum) and shares lie there too");
   static constexpr int o_scratch = stages * stage;
   static constexpr int o_vpar = o_scratch + join;                            // [warps][2][8 token pairs][NJ]{scale, min} f16x2
   static constexpr int vpar = 2 * 8 * NJ * 8;
@@ -198,6 +198,9 @@ __device__ __forceinline__ bool dc_arrive_last(int *count, int n, volatile int *
   return *s_last;
 }
 
+// Of a sum of weights (0: no token was seen), to 2 ulp.
+__device__ __forceinline__ float dc_inverse(float sum) { return sum == 0.f ? 0.f : __fdividef(1.f, sum); }
+
 // Joins n <= kDcFan partial results, each a mean of values with the reference and sum of its weights, in order;
 // sink(column, value, 4 means, reference, sum).
 template <int NJ, int NB, typename Sink>
@@ -205,9 +208,16 @@ __device__ __forceinline__ void dc_join(const float *src, int n, float *scratch,
   constexpr int D = 32 * NJ, NC = 8 * NB;
   constexpr size_t kSlot = (size_t)NC * (D + 2);
   float2 *ml = reinterpret_cast<float2 *>(scratch);   // [part][column]
+  float *share = scratch + 2 * kDcFan * NC;           // [part][column] weights, all of one reference
   dc_sync();
   for (int e = tid; e < n * NC; e += 32 * kDcWarps)
     ml[e] = __ldcg(reinterpret_cast<const float2 *>(src + (e / NC) * kSlot + (size_t)NC * D) + e % NC);
+  dc_sync();
+  for (int e = tid; e < n * NC; e += 32 * kDcWarps) {
+    float top = -INFINITY;
+    for (int c = 0; c < n; ++c) top = fmaxf(top, ml[c * NC + e % NC].x);
+    share[e] = (top == -INFINITY ? 1.f : exp2f(ml[e].x - top)) * ml[e].y;
+  }
   dc_sync();
 #pragma unroll 1
   for (int e = tid; e < NC * D / 4; e += 32 * kDcWarps) {
@@ -217,18 +227,13 @@ __device__ __forceinline__ void dc_join(const float *src, int n, float *scratch,
     for (int c = 0; c < kDcFan; ++c)
       v[c] = c < n ? __ldcg(reinterpret_cast<const float4 *>(src + c * kSlot + (size_t)col * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
     float top = -INFINITY, sum = 0.f;
-    for (int c = 0; c < n; ++c) top = fmaxf(top, ml[c * NC + col].x);
-    const auto weight = [&](int c) {
-      const float2 x = ml[c * NC + col];
-      return (top == -INFINITY ? 1.f : exp2f(x.x - top)) * x.y;
-    };
-    for (int c = 0; c < n; ++c) sum += weight(c);
-    const float r = sum == 0.f ? 0.f : 1.f / sum;
+    for (int c = 0; c < n; ++c) top = fmaxf(top, ml[c * NC + col].x), sum += share[c * NC + col];
+    const float r = dc_inverse(sum);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int c = 0; c < kDcFan; ++c) {
       if (c >= n) break;
-      const float f = weight(c) * r;
+      const float f = share[c * NC + col] * r;
       acc.x = fmaf(f, v[c].x, acc.x), acc.y = fmaf(f, v[c].y, acc.y), acc.z = fmaf(f, v[c].z, acc.z), acc.w = fmaf(f, v[c].w, acc.w);
     }
     sink(col, d, acc, top, sum);
@@ -725,7 +730,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, x);
         if (g == 0) s_m[warp * NC + col] = m[nb][c], s_l[warp * NC + col] = ls;
-        const float r = ls == 0.f ? 0.f : 1.f / ls;
+        const float r = dc_inverse(ls);
 #pragma unroll
         for (int j = 0; j < 2 * NJ; ++j)
           *reinterpret_cast<float2 *>(s_o + (warp * NC + col) * D + 32 * (j / 2) + 4 * g + 2 * (j % 2)) =
@@ -747,7 +752,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
         fl[w] = (top == -INFINITY ? 1.f : exp2f(s_m[w * NC + col] - top)) * s_l[w * NC + col];
         sum += fl[w];
       }
-      const float r = sum == 0.f ? 0.f : 1.f / sum;
+      const float r = dc_inverse(sum);
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kDcWarps; ++w) {
