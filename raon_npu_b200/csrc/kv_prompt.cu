@@ -211,7 +211,9 @@ __device__ __forceinline__ int pr_exponent(const uint32_t (&par)[NJ]) {
   }
   return e;
 }
-__device__ __forceinline__ int pr_shift(int e) { return max(-126, min(122 - e, 106)); }
+// The power that brings the largest scale below 2^-4; 2^20 of it more, which the codes take, is an f16 then.  Down to
+// -132, more than pow2f has in one factor.
+__device__ __forceinline__ int pr_shift(int e) { return min(122 - e, 106); }
 
 // Eight codes of a word into four f16x2 {nibble i, nibble i + 4}, scaled.
 __device__ __forceinline__ uint4 pr_unpack(uint32_t w, uint32_t s2, uint32_t m2) {
@@ -408,7 +410,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           __syncwarp();
           if (lane == 0) mbar_arrive(bars.s_free);
           const int4 f = info[(n + j) % kPrInfo];
-          const float c = fmaxf(crow[(k & 1) * 2 * kPrRows + t * kPrRows + row] * pow2f(-f.x), 0x1p-126f);   // above 0 (also of NaN): a hidden score is -Inf
+          const float c = fmaxf(crow[(k & 1) * 2 * kPrRows + t * kPrRows + row] * pow2f(-f.x >> 1) * pow2f(-f.x - (-f.x >> 1)), 0x1p-126f);   // above 0 (also of NaN): a hidden score is -Inf
           const int t0 = pr_block(*it, j);
           const int c_hi = pos - t0, c_lo = p.window > 0 ? c_hi - p.window : INT_MIN, c_sink = p.sinks - t0;
           if (masked) {
@@ -489,7 +491,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           const bool live = qi < it->rows_do;
           uint16_t *dst = p.out + (size_t)(it->first + qi) * p.ldo + (size_t)(it->head * p.group + flat - qi * p.group) * D;
           if (blocks && isnan(crow[(k & 1) * 2 * kPrRows + t * kPrRows + row])) nan_groups = (1u << NJ) - 1u;
-          const float r = l == 0.f ? 0.f : 1.f / l, un = pow2f(-fv);
+          const float r = (l == 0.f ? 0.f : 1.f / l) * pow2f(-(fv >> 1)), un = pow2f((fv >> 1) - fv);   // with V's power, in two factors
           const unsigned long long mine = live ? reinterpret_cast<unsigned long long>(dst) : 0ull;
           // columns 8W + 2i + o hold dim 32 (j + o) + 4 g + i, W = (g NJ + j) / 2; two of the 32-value groups at a time
 #pragma unroll 1
@@ -657,7 +659,7 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
         if (!attn_wait(bar_empty + 8 * s, ((n >> 1) & 1) ^ 1, abort, p.err)) break;
         if (!kv) tell();                                  // not before: block n - 4's may still be read
         // four words of codes at a time, each with its {scale, min}
-        const float up = pow2f(f), up20 = up * 0x1p20f;
+        const float up = pow2f(f >> 1) * pow2f(f - (f >> 1)), up20 = up * 0x1p20f;
         uint32_t s2[4], m2[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {

@@ -46,3 +46,28 @@ def test_large_values_over_many_partial_results(torch, ctx):  # noqa: F811
     c = Case(torch, ctx, 64, 1, 128, [9001], seed=30, v_scale=5e37, layers=1)
     c.layer = 0
     c.check(4)
+
+
+@pytest.mark.parametrize("qs", PROMPT)
+def test_values_up_to_the_largest_in_prompts(torch, ctx, qs):  # noqa: F811
+    values_up_to_the_largest(torch, ctx, qs)
+
+
+def keys_up_to_the_largest(torch, ctx, qs):  # noqa: F811
+    """Scales of keys past 2^122 under queries so small that the scores are ordinary ones."""
+    c = Case(torch, ctx, 64, 2, 32, [150, 105], qs, seed=23, k_scale=3e37)
+    assert (c.pool.part("k")[1][c.layer, c.table[0, 0], :, :, :, 0] >> 7).max() >= 127 + 122
+    c.check(8, q_scale=1e-37)
+
+
+@pytest.mark.parametrize("qs", PROMPT)
+def test_keys_up_to_the_largest_in_prompts(torch, ctx, qs):  # noqa: F811
+    keys_up_to_the_largest(torch, ctx, qs)
+
+
+# (queries 30 times as large are left out: the weights that this kernel takes as zero then decide elements whose other
+# values are exactly zero)
+@pytest.mark.parametrize("q_scale,k_scale,v_scale", [(1e-3, 1.0, 1e-6), (1.0, 8.0, 3e7), (1.0, 1e-4, 1e-20)])
+def test_magnitudes_of_prompts(torch, ctx, q_scale, k_scale, v_scale):  # noqa: F811
+    c = Case(torch, ctx, 64, 2, 32, [150, 105], [100, 5], seed=2, k_scale=k_scale, v_scale=v_scale)
+    c.check(8, q_scale=q_scale)
