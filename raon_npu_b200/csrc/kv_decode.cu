@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
         for (int c = 0; c < 2; ++c) {
           const int from = 4 * (2 * q4 + c), ci = attn_row(a, it.cb * NC + 8 * nb + 2 * q4 + c);
           // above 0, so that a hidden score is -Inf
-          cs[nb][c] = fmaxf(pow2f(-__shfl_sync(0xffffffffu, sh, from)) * 0x1p24f * fabsf(a.scale_log2), 0x1p-100f);
+          cs[nb][c] = fmaxf(pow2f(-__shfl_sync(0xffffffffu, sh, from)) * 0x1p24f * fabsf(a.scale_log2), 0x1p-126f);
           pos[nb][c] = ci < it.rows_do ? it.len - it.rows + ci : -1;
         }
       }

@@ -71,3 +71,8 @@ def test_keys_up_to_the_largest_in_prompts(torch, ctx, qs):  # noqa: F811
 def test_magnitudes_of_prompts(torch, ctx, q_scale, k_scale, v_scale):  # noqa: F811
     c = Case(torch, ctx, 64, 2, 32, [150, 105], [100, 5], seed=2, k_scale=k_scale, v_scale=v_scale)
     c.check(8, q_scale=q_scale)
+
+
+@pytest.mark.parametrize("qs", DECODE)
+def test_keys_up_to_the_largest(torch, ctx, qs):  # noqa: F811
+    keys_up_to_the_largest(torch, ctx, qs)
