@@ -404,7 +404,8 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int sh = top < (15u << 7) ? 126 : 141 - (int)(top >> 7);   // largest value to [2^14, 2^15)
-        const float mul = a.scale_log2 < 0.f ? -pow2f(sh) : pow2f(sh);   // the sign of the scale goes into q
+        // the sign of the scale goes into q, and a scale of zero: the factor of the scores cannot be zero
+        const float mul = a.scale_log2 < 0.f ? -pow2f(sh) : a.scale_log2 > 0.f ? pow2f(sh) : 0.f;
         uint32_t part[3][NJ];                             // group sums, 2^-24 as the codes, in three bf16
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {

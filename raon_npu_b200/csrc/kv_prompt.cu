@@ -594,8 +594,9 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
 #pragma unroll
             for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
             const int sh = top < (15u << 7) ? 126 : 141 - (int)(top >> 7);   // largest value to [2^14, 2^15)
-            // the sign of the score scale goes into Q; a row that is not finite gives NaN, not its products
-            const float mul = top >= 0x7F80u ? 0.f : p.scale_log2 < 0.f ? -pow2f(sh) : pow2f(sh);
+            // the sign of the score scale goes into Q, and a scale of zero (the factor of the scores is above zero); a row
+            // that is not finite gives NaN, not its products
+            const float mul = top >= 0x7F80u || p.scale_log2 == 0.f ? 0.f : p.scale_log2 < 0.f ? -pow2f(sh) : pow2f(sh);
             float x[8];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {

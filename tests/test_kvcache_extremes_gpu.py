@@ -76,3 +76,13 @@ def test_magnitudes_of_prompts(torch, ctx, q_scale, k_scale, v_scale):  # noqa: 
 @pytest.mark.parametrize("qs", DECODE)
 def test_keys_up_to_the_largest(torch, ctx, qs):  # noqa: F811
     keys_up_to_the_largest(torch, ctx, qs)
+
+
+@pytest.mark.parametrize("qs", [None, [3, 50], [100, 5]])
+def test_zero_and_negative_scales(torch, ctx, qs):  # noqa: F811
+    """A scale of zero weighs all visible tokens alike, whatever the keys are."""
+    c = Case(torch, ctx, 64, 2, 16, [150, 105], qs, seed=24)
+    c.check(8, scale=0.0)
+    c.check(8, scale=-0.2)
+    big = Case(torch, ctx, 64, 2, 16, [150, 105], qs, seed=25, k_scale=3e37)
+    big.check(8, scale=0.0)
