@@ -490,7 +490,8 @@ __global__ void __launch_bounds__(kPrThreads, 1) rc_kv_prompt_kernel(const __gri
           const int flat = flat0 + row, qi = attn_row(p, flat);
           const bool live = qi < it->rows_do;
           uint16_t *dst = p.out + (size_t)(it->first + qi) * p.ldo + (size_t)(it->head * p.group + flat - qi * p.group) * D;
-          if (blocks && isnan(crow[(k & 1) * 2 * kPrRows + t * kPrRows + row])) nan_groups = (1u << NJ) - 1u;
+          // a query that is not finite, unless its row is empty (any other sees its own token)
+          if (blocks && pos >= 0 && isnan(crow[(k & 1) * 2 * kPrRows + t * kPrRows + row])) nan_groups = (1u << NJ) - 1u;
           const float r = (l == 0.f ? 0.f : 1.f / l) * pow2f(-(fv >> 1)), un = pow2f((fv >> 1) - fv);   // with V's power, in two factors
           const unsigned long long mine = live ? reinterpret_cast<unsigned long long>(dst) : 0ull;
           // columns 8W + 2i + o hold dim 32 (j + o) + 4 g + i, W = (g NJ + j) / 2; two of the 32-value groups at a time

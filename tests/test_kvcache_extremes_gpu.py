@@ -86,3 +86,34 @@ def test_zero_and_negative_scales(torch, ctx, qs):  # noqa: F811
     c.check(8, scale=-0.2)
     big = Case(torch, ctx, 64, 2, 16, [150, 105], qs, seed=25, k_scale=3e37)
     big.check(8, scale=0.0)
+
+
+# ------------------------------------------------------------- non-finite --
+def test_nan_in_hidden_tokens_of_prompts(torch, ctx):  # noqa: F811
+    """The prompt kernel's rows that see a group that reads NaN are NaN, those that do not are untouched by it."""
+    c = Case(torch, ctx, 64, 2, 16, [100, 190], [20, 190], seed=4)
+    for i, t in ((0, 85), (1, 3), (1, 140)):
+        c.pool.part("v")[1][c.layer, c.table[i, t // 16], :, t % 16, 1] = 0x7FC0
+        c.pool.part("k")[1][c.layer, c.table[i, t // 16], 1, t % 16, 0] = 0x7FC0
+    c.dev_pool.copy_(torch.from_numpy(c.pool.data))
+    got, o, bar, _ = c.attend(8, window=16, sinks=2)
+    assert np.array_equal(np.isnan(got), np.isnan(o))
+    fine = ~np.isnan(o)
+    assert fine.any() and not fine.all() and (np.abs(got - o)[fine] <= bar[fine]).all()
+
+
+@pytest.mark.parametrize("qs", [[3, 9], [100, 9]])
+@pytest.mark.filterwarnings("ignore:invalid value")
+def test_queries_that_are_not_finite(torch, ctx, qs):  # noqa: F811
+    """A query head with NaN or Inf gives NaN to itself alone, and nothing to a row that sees no token."""
+    c = Case(torch, ctx, 64, 2, 16, [150, 4], qs, seed=26)
+    q = bits(c.rng.standard_normal((sum(qs), 8, 64)))
+    n = qs[0]                                              # rows n .. n + 4 stand before their sequence's first token
+    for row, head, what in ((0, 1, 0x7FC0), (2, 3, 0x7F80), (1, 6, 0xFF80), (n + 1, 0, 0x7FC0), (n + 2, 5, 0x7F80),
+                            (n + 4, 7, 0xFFFF), (n + 6, 2, 0x7FC0), (n + 8, 4, 0x7F80)):
+        q[row, head, (5 * row + head) % 64] = what
+    got, o, bar, _ = c.attend(8, q_bits=q)
+    assert np.array_equal(np.isnan(got), np.isnan(o)) and (got[n:n + 5] == 0).all()
+    assert np.isnan(got).all(-1).sum() == np.isnan(got).any(-1).sum() == 5
+    fine = ~np.isnan(o)
+    assert (np.abs(got - o)[fine] <= bar[fine]).all()
