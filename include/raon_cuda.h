@@ -416,8 +416,8 @@ int rc_kv_destroy(rc_kv *kv);
  * floor of the minimum, bf16 ceiling of (max - min) / 15 stepped up until it
  * covers the maximum, nearest code, ties to even), with the bytes of a 64-bit
  * computation, and stored at the row's position.  A group with a non-finite
- * value or a range that overflows is stored as NaN and sets the device error
- * word.  x, q_out, the norm weights and rope are 16-byte aligned. */
+ * value, or a minimum whose bf16 floor is not finite, is stored as NaN and sets
+ * the device error word.  x, q_out, the norm weights and rope are 16-byte aligned. */
 int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, int q_heads, int n_rows,
                  const int32_t *table_dev, int cols, int ld_table, const int32_t *kv_len_dev,
                  const int32_t *q_off_dev, int n_seqs, const uint16_t *q_norm_dev, const uint16_t *k_norm_dev, float eps,

@@ -138,7 +138,8 @@ __device__ __forceinline__ bool group_scale(double lo, double hi, float &sc, flo
   mn = bf16_floor_f32(__double2float_rd(lo));
   const double base = (double)mn, span = hi - base;
   // The smallest bf16 that is at least span / 15: a candidate that may be one step low, then the exact comparison.
-  sc = bf16_ceil_f32(__double2float_rn(span) * (float)(0.999999 / 15.0));
+  // The span itself may pass the largest 32-bit number, a 15th of it does not.
+  sc = bf16_ceil_f32(__double2float_rn(span * (0.999999 / 15.0)));
   if (15.0 * (double)sc < span) sc = bf16_next_up(sc);
   if (base + 15.0 * (double)sc < hi) sc = bf16_next_up(sc);   // one step covers the rounding of the sum
   if (span == 0.0) sc = 0.f;

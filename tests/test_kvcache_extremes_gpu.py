@@ -117,3 +117,26 @@ def test_queries_that_are_not_finite(torch, ctx, qs):  # noqa: F811
     assert np.isnan(got).all(-1).sum() == np.isnan(got).any(-1).sum() == 5
     fine = ~np.isnan(o)
     assert (np.abs(got - o)[fine] <= bar[fine]).all()
+
+
+# ----------------------------------------------------------------- append --
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_of_groups_wider_than_the_largest_number(torch, ctx, norm):  # noqa: F811
+    """A group from -3e38 to 3e38 has a finite scale, 4e37: it is stored as in 64 bits, without an error."""
+    c = Case(torch, ctx, 64, 2, 16, [5], seed=27, fill=False)
+    x = c.rng.standard_normal((1, 4 * 64)).astype(np.float32)
+    for at in (3, 40, 64 + 9, 128 + 33, 192 + 1):
+        x[0, at:at + 5] = [3e38, -3e38, 1e38, -2.5e38, 0.5]
+    x[0, 128 + 2:128 + 4] = [3.38e38, -3.38e38]
+    w = bits(np.full(64, 1e38)) if norm else None
+    k = x[:, :128].reshape(1, 2, 64).astype(np.float64)
+    if norm:
+        x[0, :128] = c.rng.standard_normal(128)            # its norm weight takes it there
+        k = ok.norm_rope(x[:, :128].reshape(1, 2, 64), value(w))
+    c.cache.append(0, torch.from_numpy(x).cuda(), c.batch, k_norm=None if w is None else torch.from_numpy(w.view(np.int16)).cuda())
+    torch.cuda.synchronize()
+    ctx.sync()
+    page = c.table[0, 0]
+    c.pool.store("k", 0, page, 4, k[0])
+    c.pool.store("v", 0, page, 4, x[0, 128:].reshape(2, 64).astype(np.float64))
+    assert np.array_equal(c.dev_pool.cpu().numpy(), c.pool.data)
