@@ -387,7 +387,8 @@ int rc_add_rms_bf16(rc_ctx *ctx, const uint16_t *a_dev, const uint16_t *b_dev, u
  * NULL: one row per sequence).  Row i of a sequence of n rows stands at
  * position kv_len - n + i; a row whose position is negative is empty (an idle
  * slot of a captured batch): it stores nothing and its attention is zero.
- * Rows past q_off[n_seqs] are left alone.  max_q is an upper bound of the rows
+ * Rows past q_off[n_seqs] are left alone, and a batch without rows or sequences
+ * is no work (its buffers may be NULL).  max_q is an upper bound of the rows
  * of a sequence, n_rows the rows the buffers hold.  Ids and lengths are read
  * on the device: a page id outside the pool, or a length outside the table,
  * sets the device error word (RC_ERR_INVALID at the next synchronising call)

@@ -21,7 +21,7 @@ extern "C" int rc_kv_attend(rc_kv *kv, int layer, const uint16_t *q_dev, int ldq
                             const int32_t *table_dev, int cols, int ld_table,
                             const int32_t *kv_len_dev, const int32_t *q_off_dev, int n_seqs, int max_q, float scale, int window, int sinks,
                             uint16_t *out_dev, int ldo, void *stream) {
-  RC_CHECK_ARG(kv && q_dev && out_dev, "rc_kv_attend: NULL argument");
+  RC_CHECK_ARG(kv && ((q_dev && out_dev) || n_rows == 0), "rc_kv_attend: NULL argument");
   int rc = kv_check_batch("rc_kv_attend", kv, layer, n_rows, table_dev, cols, ld_table, kv_len_dev, q_off_dev, n_seqs);
   if (rc) return rc;
   RC_CHECK_ARG(q_heads >= kv->heads && q_heads % kv->heads == 0 && q_heads <= 4096,

@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kMoveThreads) rc_kv_move_kernel(const __grid_c
 int kv_check_batch(const char *what, const rc_kv *kv, int layer, int n_rows, const int32_t *table, int cols, int ld,
                    const int32_t *kv_len, const int32_t *q_off, int n_seqs) {
   RC_CHECK_ARG(layer >= 0 && layer < kv->layers, "%s: layer %d of %d", what, layer, kv->layers);
-  RC_CHECK_ARG(table && kv_len, "%s: NULL table or kv_len", what);
+  RC_CHECK_ARG(n_seqs == 0 || (table && kv_len), "%s: NULL table or kv_len", what);
   RC_CHECK_ARG(n_seqs >= 0 && n_seqs <= kKvMaxSeqs, "%s: %d sequences (0..%d)", what, n_seqs, kKvMaxSeqs);
   RC_CHECK_ARG(n_rows >= 0, "%s: %d rows", what, n_rows);
   RC_CHECK_ARG(q_off || n_rows == n_seqs, "%s: %d rows for %d sequences without q_off", what, n_rows, n_seqs);
@@ -497,12 +497,12 @@ int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, 
                  const int32_t *q_off_dev, int n_seqs, const uint16_t *q_norm_dev, const uint16_t *k_norm_dev, float eps,
                  const float *rope_dev, int rope_rows, int rope_dim, int interleaved, uint16_t *q_out_dev, int ldq,
                  void *stream) {
-  RC_CHECK_ARG(kv && x_dev, "rc_kv_append: NULL argument");
+  RC_CHECK_ARG(kv && (x_dev || n_rows == 0), "rc_kv_append: NULL argument");
   int rc = kv_check_batch("rc_kv_append", kv, layer, n_rows, table_dev, cols, ld_table, kv_len_dev, q_off_dev, n_seqs);
   if (rc) return rc;
   RC_CHECK_ARG(x_dtype == RC_DTYPE_BF16 || x_dtype == RC_DTYPE_F32, "rc_kv_append: unknown dtype %d", x_dtype);
   RC_CHECK_ARG(q_heads >= 0 && q_heads <= 4096, "rc_kv_append: %d query heads", q_heads);
-  RC_CHECK_ARG(q_heads == 0 || q_out_dev, "rc_kv_append: q_out is NULL");
+  RC_CHECK_ARG(q_heads == 0 || n_rows == 0 || q_out_dev, "rc_kv_append: q_out is NULL");
   const long long width = (long long)(q_heads + 2 * kv->heads) * kv->dim;
   RC_CHECK_ARG(ldx >= width, "rc_kv_append: rows of %d values, %lld are needed", ldx, width);
   RC_CHECK_ARG(q_heads == 0 || ldq >= q_heads * kv->dim, "rc_kv_append: q_out rows of %d values, %d are needed", ldq,
@@ -554,7 +554,7 @@ int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, 
 
 int rc_kv_read(rc_kv *kv, int layer, int n_rows, const int32_t *table_dev, int cols, int ld_table,
                const int32_t *kv_len_dev, const int32_t *q_off_dev, int n_seqs, uint16_t *k_out_dev, uint16_t *v_out_dev, void *stream) {
-  RC_CHECK_ARG(kv && k_out_dev && v_out_dev, "rc_kv_read: NULL argument");
+  RC_CHECK_ARG(kv && ((k_out_dev && v_out_dev) || n_rows == 0), "rc_kv_read: NULL argument");
   int rc = kv_check_batch("rc_kv_read", kv, layer, n_rows, table_dev, cols, ld_table, kv_len_dev, q_off_dev, n_seqs);
   if (rc) return rc;
   RC_CHECK_ARG(aligned16(k_out_dev) && aligned16(v_out_dev), "rc_kv_read: buffers must be 16-byte aligned");

@@ -140,3 +140,27 @@ def test_append_of_groups_wider_than_the_largest_number(torch, ctx, norm):  # no
     c.pool.store("k", 0, page, 4, k[0])
     c.pool.store("v", 0, page, 4, x[0, 128:].reshape(2, 64).astype(np.float64))
     assert np.array_equal(c.dev_pool.cpu().numpy(), c.pool.data)
+
+
+# ---------------------------------------------------------- empty batches --
+@pytest.mark.parametrize("n_seqs", [0, 3])
+def test_batches_without_rows(torch, ctx, n_seqs):  # noqa: F811
+    """No sequences, or sequences without rows: nothing to do, and nothing done."""
+    from raon_npu_b200.kvcache import KvBatch
+    c = Case(torch, ctx, 64, 2, 16, [20, 30, 7], seed=28)
+    before = c.dev_pool.clone()
+    empty = lambda *s: torch.empty((0, *s), dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    batches = [KvBatch(c.dev_table[:n_seqs], c.kv_len[:n_seqs], torch.zeros(n_seqs + 1, dtype=torch.int32, device="cuda"))]
+    if n_seqs == 0:
+        batches += [KvBatch(c.dev_table[:0], c.kv_len[:0]), c.cache.batch([])]
+    else:
+        seqs = [c.cache.new() for _ in range(n_seqs)]
+        c.cache.extend(seqs, 5)
+        batches.append(c.cache.batch(seqs, rows=[0] * n_seqs))
+    for batch in batches:
+        c.cache.append(0, empty(8 * 64), batch, empty(4 * 64), q_heads=4)
+        c.cache.attend(0, empty(4 * 64), batch, empty(4, 64))
+        c.cache.read(0, batch, empty(2, 64), empty(2, 64))
+    torch.cuda.synchronize()
+    ctx.sync()
+    assert torch.equal(before, c.dev_pool)
