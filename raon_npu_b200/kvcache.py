@@ -98,6 +98,9 @@ class KvBatch:
             _ints(q_off, 1, "q_off")
             if int(q_off.shape[0]) != self.n_seqs + 1:
                 raise ValueError(f"q_off has {q_off.shape[0]} entries for {self.n_seqs} sequences")
+        dev = table.get_device()
+        if kv_len.get_device() != dev or (q_off is not None and q_off.get_device() != dev):
+            raise ValueError(f"table, kv_len and q_off must be on one device, cuda:{dev} as the table")
         if max_q < 1 or (q_off is None and max_q != 1):
             raise ValueError(f"max_q {max_q}: at least 1, and 1 without q_off")
         self.max_q = int(max_q)
@@ -258,6 +261,8 @@ class KvCache:
         rows = cols = ld = 0
         if table is not None:
             _ints(table, 2, "table")
+            if table.get_device() != self.ctx.device:
+                raise ValueError(f"move_pages: the table must be on cuda:{self.ctx.device}")
             rows, cols = table.shape
             ld = table.stride(0) if rows > 1 else cols
         if src.get_device() != self.ctx.device or dst.get_device() != self.ctx.device:

@@ -5,10 +5,11 @@ from __future__ import annotations
 from types import SimpleNamespace
 
 import pytest
+import torch
 
 from raon_npu_b200 import kvcache
 from raon_npu_b200.build import build
-from raon_npu_b200.kvcache import KvCache, PagePool
+from raon_npu_b200.kvcache import KvBatch, KvCache, PagePool
 
 
 class Ids:
@@ -54,3 +55,55 @@ def test_the_moves_of_a_call_outlive_its_launch(monkeypatch, op, stream, waits_f
         pool.free(a)
         assert cache.compact(stream=stream) == 1
     assert launched == [(waits_for, stream)]
+
+
+# ---------------------------------------------------------------- devices --
+class Ints:
+    """An int32 tensor on some GPU."""
+
+    dtype, is_cuda = torch.int32, True
+
+    def __init__(self, device, *shape, strides=None):
+        self.device, self.shape = torch.device("cuda", device), torch.Size(shape)
+        self.strides = strides or torch.empty(shape, device="meta").stride()
+
+    def dim(self):
+        return len(self.shape)
+
+    def stride(self, i=None):
+        return self.strides if i is None else self.strides[i]
+
+    def get_device(self):
+        return self.device.index
+
+    def data_ptr(self):
+        return 16
+
+
+def stand_in_cache(launched=None):
+    """A cache on GPU 0 without its handle; ``launched`` takes what reaches rc_kv_move_pages."""
+    cache = KvCache.__new__(KvCache)
+    cache.ctx, cache.device, cache.handle = SimpleNamespace(device=0, handle=None), 0, None
+    cache.lib = SimpleNamespace(rc_kv_move_pages=lambda *a: launched.append(a) or 0)
+    return cache
+
+
+def test_the_arrays_of_a_batch_are_on_one_gpu():
+    ok = KvBatch(Ints(1, 2, 3), Ints(1, 2), Ints(1, 3), max_q=4)
+    assert (ok.n_seqs, ok.columns, ok.ld) == (2, 3, 3)
+    for table, kv_len, q_off in ((0, 1, None), (1, 0, 1), (0, 0, 1), (1, 1, 0)):
+        with pytest.raises(ValueError, match="one device"):
+            KvBatch(Ints(table, 2, 3), Ints(kv_len, 2), None if q_off is None else Ints(q_off, 3), 1)
+    with pytest.raises(ValueError, match="the batch is on cuda:1"):
+        stand_in_cache()._batch_args(ok, 2, "attend")
+
+
+def test_the_arrays_of_a_move_are_on_the_caches_gpu():
+    launched = []
+    cache = stand_in_cache(launched)
+    for src, dst, table in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, None)):
+        with pytest.raises(ValueError, match="cuda:0"):
+            cache.move_pages(Ints(src, 4), Ints(dst, 4), table=None if table is None else Ints(table, 2, 5), stream=7)
+    assert not launched
+    cache.move_pages(Ints(0, 4), Ints(0, 4), table=Ints(0, 2, 5, strides=(8, 1)), stream=7)
+    assert launched == [(None, 16, 16, 4, 16, 2, 5, 8, 7)]
