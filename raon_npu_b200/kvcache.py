@@ -19,6 +19,7 @@ Buffers are torch tensors on the context's device; 16-bit rows may be
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import numpy as np
 import torch
@@ -72,6 +73,14 @@ def _rows(t, width: int, what: str, dev: int, types=_BF16):
     if ld < width:
         raise ValueError(f"{what}: rows overlap (stride {ld} of {width} values)")
     return rows, ld
+
+
+def _whole(numbers, what: str) -> np.ndarray:
+    """int32 array of whole numbers of any integer type."""
+    try:
+        return np.asarray([operator.index(n) for n in numbers], dtype=np.int32)
+    except (TypeError, OverflowError) as e:
+        raise ValueError(f"{what} must be whole 32-bit numbers: {e}") from None
 
 
 class KvBatch:
@@ -315,7 +324,7 @@ class KvCache:
         dev = torch.device("cuda", self.ctx.device)
         q_off, max_q = None, 1
         if rows is not None:
-            rows = np.asarray(list(rows), dtype=np.int64)
+            rows = _whole(rows, "batch: rows")
             if rows.shape != kv_len.shape or (rows < 0).any() or (rows > kv_len).any():
                 raise ValueError("batch: rows must be between 0 and each sequence's tokens")
             q_off = torch.from_numpy(np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)).to(dev)
@@ -356,8 +365,9 @@ class PagePool:
     def extend(self, seqs, n) -> list[tuple[int, int]]:
         """n more tokens (a number, or one for each) for every sequence; the (source, destination) page copies to
         launch before anything is written to them."""
-        ids = np.asarray(list(seqs), dtype=np.int32)
-        counts = np.full(len(ids), n, np.int32) if isinstance(n, int) else np.asarray(list(n), dtype=np.int32)
+        ids = _whole(seqs, "extend: sequences")
+        one = not hasattr(n, "__iter__") or getattr(n, "ndim", 1) == 0
+        counts = _whole([n] * len(ids) if one else n, "extend: counts")
         if counts.shape != ids.shape:
             raise ValueError(f"extend: {len(ids)} sequences, {len(counts)} counts")
         src, dst, k = np.empty(len(ids), np.int32), np.empty(len(ids), np.int32), ctypes.c_int()
@@ -396,7 +406,7 @@ class PagePool:
 
     def table(self, seqs, columns: int | None = None) -> tuple[np.ndarray, np.ndarray]:
         """int32 [sequences, columns] page ids (-1 past a sequence's pages) and int32 token counts."""
-        ids = np.asarray(list(seqs), dtype=np.int32)
+        ids = _whole(seqs, "table: sequences")
         if columns is None:
             columns = max([1] + [-(-self.tokens(int(s)) // self.page_size) for s in ids])
         table, kv_len = np.empty((len(ids), columns), np.int32), np.empty(len(ids), np.int32)

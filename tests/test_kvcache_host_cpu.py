@@ -4,6 +4,7 @@ from __future__ import annotations
 
 from types import SimpleNamespace
 
+import numpy as np
 import pytest
 import torch
 
@@ -107,3 +108,29 @@ def test_the_arrays_of_a_move_are_on_the_caches_gpu():
     assert not launched
     cache.move_pages(Ints(0, 4), Ints(0, 4), table=Ints(0, 2, 5, strides=(8, 1)), stream=7)
     assert launched == [(None, 16, 16, 4, 16, 2, 5, 8, 7)]
+
+
+# ---------------------------------------------------------------- numbers --
+@pytest.mark.parametrize("one", [3, np.int64(3), np.int32(3), np.array(3), torch.tensor(3)])
+def test_counts_of_any_integer_type(one):
+    build()
+    pool = PagePool(8, 4)
+    a, b = pool.new(), pool.new()
+    pool.extend([a, b], one)
+    pool.extend(np.array([a, b]), [one, 1])
+    pool.extend(torch.tensor([b]), np.array([2]))
+    assert [pool.tokens(a), pool.tokens(b)] == [6, 6]
+
+
+@pytest.mark.parametrize("bad", [1.5, [1.0], "1", None, 2**31, [2**40]])
+def test_counts_that_are_not_whole_numbers_are_refused(bad):
+    build()
+    pool = PagePool(8, 4)
+    a = pool.new()
+    with pytest.raises(ValueError):
+        pool.extend([a], bad)
+    with pytest.raises(ValueError):
+        pool.extend([0.5], 1)
+    with pytest.raises(ValueError):
+        pool.table([0.5])
+    assert pool.tokens(a) == 0
