@@ -59,10 +59,28 @@ constexpr int kDcMinStages = 4, kDcMaxStages = 6, kDcMaxChunks = 256;
 constexpr int kDcFan = 16;                        // partial results joined at a time
 constexpr int kDcGroups = (kDcMaxChunks + kDcFan - 1) / kDcFan;
 
+__host__ __device__ constexpr int dc_min(int a, int b) { return a < b ? a : b; }
+__host__ __device__ constexpr int dc_max(int a, int b) { return a > b ? a : b; }
+__host__ __device__ constexpr int dc_ceil(int a, int b) { return (a + b - 1) / b; }
+// Stages of a chunk of a sequence of ``stages``.
+__host__ __device__ constexpr int dc_per_chunk(int stages) {
+  return dc_max(dc_min(dc_max(dc_ceil(stages, 8), kDcMinStages), kDcMaxStages), dc_ceil(stages, kDcMaxChunks));
+}
+// The most chunks of a sequence of up to ``stages``: eight while they grow, then those of the largest constant chunk.
+__host__ __device__ constexpr int dc_most_chunks(int stages) {
+  return dc_max(dc_min(dc_ceil(stages, kDcMinStages), 8), dc_min(dc_ceil(stages, kDcMaxStages), kDcMaxChunks));
+}
+constexpr bool dc_holds(int stages) {
+  for (int s = 1; s <= stages; ++s)
+    if (dc_ceil(s, dc_per_chunk(s)) > dc_most_chunks(s) || dc_most_chunks(s) < dc_most_chunks(s - 1)) return false;
+  return true;
+}
+static_assert(dc_holds(4 * kDcMaxChunks * kDcMaxStages), "the partial results of a sequence have room");
+
 struct DcParams {
   AttnParams a;
   int cbs;            // column blocks of max_q rows
-  int slots;          // partials of one (sequence, head, column block): its chunks', then its groups'
+  int chunks, slots;  // partials of one (sequence, head, column block): its chunks', then, if any, its groups'
   float *part;        // [n_seqs][heads][cbs][slots][cols * (D + 2)]
   int *count;         // [n_seqs][heads][cbs][1 + groups] arrivals, zero between launches
 };
@@ -83,7 +101,7 @@ __device__ __forceinline__ DcSeq dc_seq(const AttnParams &p, int b) {
   const int first = s.lo / kDcStage;
   s.n_sink = min((s.sinks + kDcStage - 1) / kDcStage, first);
   s.stages = s.n_sink + (s.len + kDcStage - 1) / kDcStage - first;
-  s.per_chunk = max(min(max((s.stages + 7) / 8, kDcMinStages), kDcMaxStages), (s.stages + kDcMaxChunks - 1) / kDcMaxChunks);
+  s.per_chunk = dc_per_chunk(s.stages);
   s.n_chunks = max(1, (s.stages + s.per_chunk - 1) / s.per_chunk);
   return s;
 }
@@ -782,7 +800,7 @@ __global__ void __launch_bounds__(kDcThreads, NB == 1 ? 3 : 2) rc_kv_decode_kern
             attn_write4(a, it.first, it.rows_do, it.cb * NC + col, it.head, D, d, acc);
           });
         } else {
-          float *mid = cell_part + (size_t)(p.slots - kDcGroups) * kSlot;
+          float *mid = cell_part + (size_t)p.chunks * kSlot;
           dc_join<NJ, NB>(src, n, s_o, tid, [&](int col, int d, float4 acc, float top, float sum) {
             float *dst = mid + grp * kSlot;
             __stcg(reinterpret_cast<float4 *>(dst + (size_t)col * D + d), acc);
@@ -803,9 +821,9 @@ static int decode_launch(rc_ctx *ctx, DcParams &p, int max_q, cudaStream_t s) {
   using L = DcLayout<NJ, NB>;
   const AttnParams &a = p.a;
   const long long stages = ((long long)a.b.cols * a.g.page + kDcStage - 1) / kDcStage + 1;   // one more: a window cuts two
-  const long long chunks = (stages + kDcMinStages - 1) / kDcMinStages;
   p.cbs = (int)(((long long)max_q * a.group + L::cols - 1) / L::cols);
-  p.slots = (int)(chunks < kDcMaxChunks ? chunks : kDcMaxChunks) + kDcGroups;
+  p.chunks = stages < 2 * kDcMaxChunks * kDcMaxStages ? dc_most_chunks((int)stages) : kDcMaxChunks;
+  p.slots = p.chunks + (p.chunks > kDcFan ? dc_ceil(p.chunks, kDcFan) : 0);
   const long long cells = (long long)a.b.n_seqs * a.g.heads * p.cbs;
   RC_CHECK_ARG(cells * (stages + kDcMaxChunks) <= INT_MAX, "rc_kv_attend: the batch is too large");
   int rc = ensure_attn_scratch(ctx, (size_t)cells * p.slots * L::cols * (L::D + 2) * sizeof(float), (size_t)cells * (kDcGroups + 1));
@@ -823,7 +841,7 @@ static int decode_launch(rc_ctx *ctx, DcParams &p, int max_q, cudaStream_t s) {
     RC_CHECK_ARG(per_sm >= 1, "rc_kv_attend: the decode kernel does not fit an SM");
     if (ctx->device < 64) resident[ctx->device][bucket].store(per_sm, std::memory_order_relaxed);
   }
-  const long long items = cells * (p.slots - kDcGroups), cap = (long long)ctx->sm_count * per_sm;
+  const long long items = cells * p.chunks, cap = (long long)ctx->sm_count * per_sm;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(items < cap ? items : cap));
   cfg.blockDim = dim3(kDcThreads);

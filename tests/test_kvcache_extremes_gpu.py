@@ -164,3 +164,28 @@ def test_batches_without_rows(torch, ctx, n_seqs):  # noqa: F811
     torch.cuda.synchronize()
     ctx.sync()
     assert torch.equal(before, c.dev_pool)
+
+
+# ---------------------------------------------------------------- scratch --
+@pytest.mark.parametrize("tokens,chunks,groups", [(131072, 171, 11), (8192, 11, 0), (896, 2, 0)])
+def test_scratch_holds_what_the_table_can_ask_for(torch, ctx, tokens, chunks, groups):  # noqa: F811
+    """64 sequences of 8 kv heads: room for the chunks that a sequence as long as its table row has (of six stages of 128
+    tokens from 48 stages on, eight or fewer below), and no more than rounding beside it."""
+    from raon_npu_b200.device import Context
+    from raon_npu_b200.kvcache import KvBatch, KvCache
+    own = Context(0)
+    cache = KvCache(own, 1, 8, 128, 64, page_size=128)
+    table = torch.arange(64, dtype=torch.int32, device="cuda").reshape(64, 1).repeat(1, tokens // 128)
+    batch = KvBatch(table, torch.full((64,), 77, dtype=torch.int32, device="cuda"))
+    x = torch.randn((64, 24 * 128), device="cuda").bfloat16()
+    q, out = torch.zeros((64, 8 * 128), device="cuda").bfloat16(), torch.zeros((64, 8 * 128), device="cuda").bfloat16()
+    cache.append(0, x, batch, q, q_heads=8)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    cache.attend(0, q, batch, out)
+    torch.cuda.synchronize()
+    used = free - torch.cuda.mem_get_info()[0]
+    assert used <= 64 * 8 * (chunks + groups) * 8 * 130 * 4 + (4 << 20)
+    own.sync()
+    cache.close()
+    own.close()
