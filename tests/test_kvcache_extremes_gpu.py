@@ -189,3 +189,75 @@ def test_scratch_holds_what_the_table_can_ask_for(torch, ctx, tokens, chunks, gr
     own.sync()
     cache.close()
     own.close()
+
+
+# ------------------------------------------------- bounds, many, far away --
+@pytest.mark.parametrize("max_q", [1, 50, 70])
+def test_a_bound_of_rows_that_does_not_hold(torch, ctx, max_q):  # noqa: F811
+    """More rows than max_q says: those within it are computed, the others left alone, and the next synchronising call
+    says so, in both kernels."""
+    from raon_npu_b200.kvcache import KvBatch
+    c = Case(torch, ctx, 64, 2, 16, [120, 90], [100, 80], seed=29)
+    q = torch.randn((180, 8, 64), device="cuda").bfloat16()
+    whole, out = torch.zeros_like(q), torch.full_like(q, 7.0)
+    c.cache.attend(1, q, c.batch, whole)
+    torch.cuda.synchronize()
+    ctx.sync()
+    c.cache.attend(1, q, KvBatch(c.dev_table, c.kv_len, c.q_off, max_q), out)
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="outside"):
+        ctx.sync()
+    ctx.sync()
+    for first, rows in ((0, 100), (100, 80)):
+        assert (out[first + max_q:first + rows] == 7).all()
+        assert torch.isfinite(out[first:first + max_q].float()).all()
+        if max_q == 70:                                    # the same kernel
+            assert torch.equal(out[first:first + max_q], whole[first:first + max_q])
+
+
+@pytest.mark.parametrize("n,most", [(70, 1), (300, 1), (45, 9), (70, 60)])
+def test_many_sequences(torch, ctx, n, most):  # noqa: F811
+    """Sequences past every 32nd and 256th, of one row, a few, and enough for the prompt kernel; some without rows."""
+    rng = np.random.default_rng(n + most)
+    qs = rng.integers(0, most + 1, n)
+    qs[[0, 31, 32]] = 0, most, 0
+    lens = qs + rng.integers(0, 30, n)
+    lens[5] = 0 if most == 1 else max(1, qs[5] // 2)       # idle, or rows before the first token
+    c = Case(torch, ctx, 64, 1, 16, lens.tolist(), qs.tolist(), seed=31)
+    c.check(8)
+    c.check(8, window=9, sinks=2)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_pages_past_four_gigabytes(torch, ctx, rows):  # noqa: F811
+    """The last pages and the last layer of a pool of 6.6 GB give what the first ones give, after an append and a move."""
+    from raon_npu_b200.kvcache import KvBatch, KvCache
+    pages = 20000
+    cache = KvCache(ctx, 2, 8, 128, pages, page_size=128)
+    kv_len = torch.tensor([300, 17 + rows], dtype=torch.int32, device="cuda")
+    x = torch.randn((2 * rows, 48 * 128), device="cuda").bfloat16()
+    past = torch.randn((317 + rows, 48 * 128), device="cuda").bfloat16()
+    outs = []
+    for layer, first in ((0, 0), (1, pages - 8)):
+        table = torch.arange(first, first + 8, dtype=torch.int32, device="cuda").reshape(2, 4).flip(1).contiguous()
+        q = torch.empty((317 + rows, 32 * 128), device="cuda").bfloat16()
+        whole = KvBatch(table, kv_len, torch.tensor([0, 300, 317 + rows], dtype=torch.int32, device="cuda"), 300)
+        cache.append(layer, past, whole, q, q_heads=32)
+        batch = KvBatch(table, kv_len, torch.arange(0, 2 * rows + 1, rows, dtype=torch.int32, device="cuda"), rows)
+        q = q[:2 * rows]
+        cache.append(layer, x, batch, q, q_heads=32)
+        out = torch.zeros_like(q)
+        cache.attend(layer, q, batch, out)
+        kv = [torch.zeros((317 + rows, 8, 128), device="cuda").bfloat16() for _ in "kv"]
+        cache.read(layer, whole, *kv)
+        other = table + (8 if first == 0 else -8)
+        cache.move_pages(table.reshape(-1), other.reshape(-1).contiguous(), table=table)
+        moved = torch.zeros_like(q)
+        cache.attend(layer, q, batch, moved)
+        assert torch.equal(table, other) and torch.equal(moved, out) and out.float().abs().sum() > 0
+        outs.append([q.clone(), out, *kv])
+    torch.cuda.synchronize()
+    ctx.sync()
+    for low, high in zip(*outs):
+        assert torch.equal(low, high)
+    cache.close()
