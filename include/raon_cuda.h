@@ -386,7 +386,8 @@ int rc_add_rms_bf16(rc_ctx *ctx, const uint16_t *a_dev, const uint16_t *b_dev, u
  * q_off [n_seqs + 1] (the rows of sequence s are q_off[s] .. q_off[s+1]-1;
  * NULL: one row per sequence).  Row i of a sequence of n rows stands at
  * position kv_len - n + i; a row whose position is negative is empty (an idle
- * slot of a captured batch): it stores nothing and its attention is zero.
+ * slot of a captured batch): it stores no key or value, its query is written
+ * without a rotation and its attention is zero.
  * Rows past q_off[n_seqs] are left alone, and a batch without rows or sequences
  * is no work (its buffers may be NULL).  max_q is an upper bound of the rows
  * of a sequence, n_rows the rows the buffers hold.  Ids and lengths are read
@@ -434,9 +435,13 @@ int rc_kv_append(rc_kv *kv, int layer, const void *x_dev, int x_dtype, int ldx, 
  * At most 256 query heads share a kv head, and max_q * q_heads / kv_heads is
  * at most 2^24.  A row's bytes do not depend on the other sequences of the
  * batch, for one max_q: up to 255 rows (max_q * q_heads / kv_heads) a kernel
- * that keeps every weight, above it one that takes weights below 2^-31 of the
- * largest as zero.  Values are rounded to 11 bits or more before the products;
- * scores, sums and results are 32-bit.  Scratch grows on the first call for a
+ * that keeps weights down to 2^-64 of the largest, above it one that takes those
+ * below 2^-31 as zero.  Scores, sums and results are 32-bit.  Operands of the
+ * products that have no exact f16 are rounded to it: weights (to 11 bits, fewer
+ * below 2^-21 of the largest), values, and above 255 rows keys (to 11 bits, or
+ * to 2^-20 of the largest scale among the sequence's visible values, or among
+ * the keys of the same 128 tokens, where that is coarser).  A query value of
+ * 2^118 or more may give NaN.  Scratch grows on the first call for a
  * larger batch or table (that call allocates and synchronises the device, so it
  * must come before the call is captured) and belongs to the context: keep its
  * calls on one stream at a time.  Scratch that a captured call uses lives as

@@ -6,15 +6,19 @@ using namespace rc;
 // Rows of a sequence and kv head above which a call goes to the tensor-memory
 // kernel.  The decode kernel reads the cache once per 16 rows, split over as many
 // CTAs as there are; the other one once per 256, by one CTA a kv head.  Which is
-// faster turns on the number of sequences, and a row's bytes must not, so the rule
-// is on the rows alone, and where both sides lose alike.  us, decode / prompt, 4096
-// tokens, heads of 128:
-//                     1 sequence of 4 kv heads   of 16 kv heads   8 of 4 kv heads
-//    32 rows                  19.6 / 58.1          20.6 / 58.7       33.5 / 59.5
-//   128 rows                  20.6 / 58.7          59.1 / 59.4       95.2 / 60.7
-//   256 rows                  32.9 / 70.2          94.6 / 71.1      181.1 / 71.4
-//  1024 rows                  94.2 / 70.7                           705.1 / 75.8
-// The decode kernel also keeps weights below 2^-31 of the largest.
+// faster turns on the number of sequences and kv heads, and a row's bytes must not,
+// so the rule is on the rows alone.  us, decode / prompt, 4096 tokens, heads of 128:
+//               1 sequence, 4 kv heads   1, 16 kv heads   8, 4 kv heads   8, 16 kv heads
+//    16 rows           16.8 / 57.3         19.2 / 58.0      20.0 / 58.6      57.3 / 60.5
+//    32 rows           17.8 / 57.5         19.8 / 57.9      32.5 / 58.7      95.1 / 60.9
+//    64 rows           19.2 / 57.5         32.2 / 58.1      57.7 / 59.0     182.8 / 61.4
+//   128 rows           19.7 / 58.0         57.4 / 58.5      93.0 / 59.8     360.4 / 63.0
+//   256 rows           32.1 / 67.0         93.3 / 68.2     179.4 / 69.6     710.0 / 74.2
+//  1024 rows           92.7 / 67.8        358.5 / 69.5     700.7 / 73.1    2832.9 / 248.5
+// 255 favours single sequences and few heads (two to three times faster up to there)
+// at the price of batches: they cross at 64 rows for 8 sequences of 4 kv heads, at 16
+// for 8 of 16, which lose near ten times just below the limit.  The decode kernel also
+// keeps weights below 2^-31 of the largest.
 constexpr long long kPromptRows = 255;
 
 extern "C" int rc_kv_attend(rc_kv *kv, int layer, const uint16_t *q_dev, int ldq, int q_heads, int n_rows,

@@ -20,10 +20,12 @@ namespace rc {
 // before a long one (keys) ends: with the read-back below, 4096 rows of 32 + 4 + 4
 // heads of 128 took 47 us so, with blocks of two warps 50 and of eight 65.
 // Measured: those rows in 30 us (86 MB in and out: 2.9 TB/s, 45% of the copy rate)
-// and 10 for the read-back; 16 rows of a decode step in 5.2 us with it.  Bound by
-// instruction issue (0.60 a cycle with 19 warps an SM; 250 for a unit of 256
-// values) and, with few rows, by four dependent loads: the row's sequence, its page
-// and rotation, the values.
+// and 10 for the read-back; 16 rows of a decode step in 5.3 us with it.  Neither
+// memory (15% of its cycles) nor issue (0.60 a cycle, 250 instructions for a unit of
+// 256 values) is full: 19 warps an SM do not cover the latency of a unit's steps, the
+// 64-bit ones above all, and with few rows that of four dependent loads: the row's
+// sequence, its page and rotation, the values.  The forms for f32 rows spill 72 bytes
+// a thread (in 80 registers).
 constexpr int kAppendUnits = 4, kAppendCtas = 24;
 
 struct AppendParams {

@@ -18,7 +18,9 @@
 // code in one rounding (the code again as a subnormal operand of the packed
 // multiply-add), and P is f16 too: 2^-12 of a term each, the only roundings
 // below 32 bits.  V is brought to about 1 at most by a power of two that follows
-// the largest scale seen.  Its codes are read in the transposed fragment order
+// the largest scale seen, so a value below 2^-9 of that scale has fewer bits (it
+// is good to 2^-20 of the scale); P has 7 bits at least, and weights below 2^-64
+// of a reference are zero.  Its codes are read in the transposed fragment order
 // by byte permutes of two tokens' words, P is transposed in registers (movmatrix).
 // The softmax reference of a column moves only when a score passes it by 8
 // (in powers of two), so the sums are rescaled a few times a chunk at most.
@@ -35,10 +37,13 @@
 // chunk order.
 //
 // Measured (32 query heads, 4 kv heads of 128): 64 sequences of 65 to 8191 tokens
-// 62.6 us (170 MB: 2.7 TB/s, 42% of the copy rate), two of 111870 and 131072 tokens
-// 53.8 us (156 MB, 45%), one of 333 tokens 7.9 us.  Bound by instruction issue: 0.51
-// a cycle from 13 warps an SM, which is what the registers allow; the unpacking of
-// the codes is about half of it.
+// 62.4 us (170 MB: 2.7 TB/s, 43% of the copy rate), two of 111870 and 131072 tokens
+// 52.8 us (156 MB, 46%), one of 333 tokens 7.7 us.  Neither memory (a third of its
+// cycles) nor issue (0.53 a cycle) is full: the registers allow three computing warps
+// a scheduler, and these do not cover one another's chains of dependent steps (codes,
+// score products, weights, value products).  450 warp instructions for 16 tokens of a
+// kv head, a third of them to unpack the codes.  The forms for heads of 128 spill 12
+// to 144 bytes a thread.
 #include <limits.h>
 
 #include "kv_attn.cuh"

@@ -24,17 +24,21 @@
 // a power of two per row, K per block and V by a power of two that follows the
 // largest scale seen, so that range is not lost; O is rescaled when that power
 // or a row's softmax reference moves, the latter only when a score passes it by
-// 8 in powers of two.  Weights below 2^-31 of the reference count as zero.
+// 8 in powers of two.  A key below 2^-9 of the largest scale of its block, and a
+// value below 2^-9 of the largest seen, has fewer bits: it is good to 2^-20 of that
+// scale.  Weights below 2^-21 of the reference have fewer bits (good to 2^-32 of it),
+// and below 2^-31 they count as zero, while the sum of the weights has them all.
 // K's values keep the order of the packed row (Q is permuted alike); V's too
 // (the results are put in order on the way out).
 //
 // A V group that holds NaN is zero in the product and reaches the rows that
 // see its token by hand, so that 0 * NaN does not reach the others.
 //
-// Measured: 4096 rows of 32 heads over 4 kv heads of 128, causal, 141 us: 977
-// TFLOP/s of visible pairs, 59% of the matrix peak; chunks of 2048 and 1416 rows of
-// 32 heads over 8 that see 4096 tokens and 16 sinks 229 us (62%); six prompts of 117
-// to 701 tokens, 16 heads of 64, 20 us.  Bound by the chain of a block: scores (640
+// Measured: 4096 rows of 32 heads over 4 kv heads of 128, causal, 142 us in a graph
+// of 30 calls (970 TFLOP/s of visible pairs, 59% of the matrix peak) and 158 after a
+// tenth of a second of them, at the power cap (872; 1.73 GHz); chunks of 2048 and 1416 rows of 32 heads over 8 that
+// see 4096 tokens and 16 sinks 230 us (61%) and 259; six prompts of 117 to 701
+// tokens, 16 heads of 64, 20 us.  Bound by the chain of a block: scores (640
 // cycles), their way into registers (300), maximum (500), weights (1700; without the
 // exponentials the prompt took 125 us, without making K and V 132, with half the
 // products 141), values (530).  S and P in one place, and S for each tile, was

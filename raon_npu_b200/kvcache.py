@@ -13,7 +13,13 @@ passes them to ``KvBatch``.
 
 Buffers are torch tensors on the context's device; 16-bit rows may be
 ``torch.bfloat16`` or bf16 bits in an integer type.  Launches go to ``stream``
-(default: the current torch stream) and return at once.
+(a raw handle; default: the current torch stream) and return at once.  Tensors
+passed with a ``stream`` that is not the current one must stay alive until it
+has used them (``Tensor.record_stream``).
+
+``attend`` uses scratch of the context: calls of one context that may run at
+the same time, on two streams or in two graphs, give wrong results.  Order
+them, or give each stream a ``Context`` and a ``KvCache`` on one ``pool``.
 """
 
 from __future__ import annotations
@@ -228,7 +234,8 @@ class KvCache:
 
         scale: of the scores (default 1 / sqrt(head_dim)).  window > 0: a row
         sees itself, the window - 1 tokens before it and the first ``sinks``
-        tokens of its sequence; 0: every token up to itself."""
+        tokens of its sequence; 0: every token up to itself.  One call of a
+        context at a time, whatever the streams."""
         dev = self.device
         shape = q.shape
         width = shape[1] if len(shape) == 2 else shape[1] * shape[2] if len(shape) == 3 else 0
