@@ -36,14 +36,14 @@
 //
 // Measured: 4096 rows of 32 heads over 4 kv heads of 128, causal, 142 us in a graph
 // of 30 calls (970 TFLOP/s of visible pairs, 59% of the matrix peak) and 158 after a
-// tenth of a second of them, at the power cap (872; 1.73 GHz); chunks of 2048 and 1416 rows of 32 heads over 8 that
-// see 4096 tokens and 16 sinks 230 us (61%) and 259; six prompts of 117 to 701
-// tokens, 16 heads of 64, 20 us.  Bound by the chain of a block: scores (640
-// cycles), their way into registers (300), maximum (500), weights (1700; without the
-// exponentials the prompt took 125 us, without making K and V 132, with half the
-// products 141), values (530).  S and P in one place, and S for each tile, was
-// slower (188 us): then a tile's chain has no overlap.  A short prompt pays 7 us
-// before its first score: items, rows, codes.
+// tenth of a second of them, at the power cap (872; 1.73 GHz); chunks of 2048 and
+// 1416 rows of 32 heads over 8 that see 4096 tokens and 16 sinks 230 us (61%) and
+// 259; six prompts of 117 to 701 tokens, 16 heads of 64, 20 us.  Bound by the chain
+// of a block: scores (640 cycles), their way into registers (300), maximum (500),
+// weights (1700; without the exponentials the prompt took 125 us, without making K
+// and V 132, with half the products 141), values (530).  S and P in one place, and S
+// for each tile, was slower (188 us): then a tile's chain has no overlap.  A short
+// prompt pays 7 us before its first score: items, rows, codes.
 #include <limits.h>
 
 #include "kv_attn.cuh"

@@ -261,3 +261,21 @@ def test_pages_past_four_gigabytes(torch, ctx, rows):  # noqa: F811
     for low, high in zip(*outs):
         assert torch.equal(low, high)
     cache.close()
+
+
+# -------------------------------------------------------------- precision --
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("qs", [None, [40, 7], [150, 40]])
+def test_the_noise_is_that_of_operands_of_eleven_bits(torch, ctx, d, qs):  # noqa: F811
+    """The outputs' error in root mean square, against the rounding to bf16 and 2^-11 of ``noise``: weights, values and (in
+    prompts) keys are each off by up to 2^-12, evenly spread, which is 2^-12 of ``noise`` for the three together, and
+    twice that is allowed.  Operands of nine bits would have four times as much."""
+    lens = [400, 333]
+    c = Case(torch, ctx, d, 2, 64, lens, qs, seed=d)
+    got, o, _, q = c.attend(4 * 2)
+    noise = np.zeros_like(o)
+    for i, n in enumerate(c.qs):
+        a = slice(c.off[i], c.off[i] + n)
+        noise[a] = ok.attend(value(q[a]), *c.kv(i), lens[i] - n)[1]
+    rms = lambda x: np.sqrt((x * x).mean())  # noqa: E731
+    assert rms(got - o) ** 2 <= rms(ok.bf16(o) - o) ** 2 * 1.01 + (2.0**-11 * rms(noise)) ** 2
